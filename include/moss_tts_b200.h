@@ -355,6 +355,70 @@ int mt_prefill_attention(const void* q, const void* k_cache, const void* v_cache
                          int nq, int nkv, int max_len, int flags, void* stream);
 
 /*
+ * A paged key-value cache of one layer, for the four calls below (no counterpart in the reference,
+ * whose cache is one contiguous buffer for one sequence, src/moss_tts/_runtime/llm.py:166-172).
+ * Key j of sequence b lies in row j % page_size of page page_table[b][j / page_size]:
+ *   k_pages[page][head][row][head_dim], likewise v_pages; the strides of a page, a head and a row
+ *   are in elements, multiples of 8; the head_dim elements of a row are adjacent.
+ * page_table int32 [batch][max_pages], rows table_stride elements apart; kv_lens int32 [batch], the
+ * tokens of each sequence, the new ones included. type 0 = bf16, 1 = fp16; head_dim 64 or 128;
+ * page_size a power of two, 16 to 256; 16-byte aligned pages. The struct itself is read on the host
+ * during the call.
+ * `status` (int32, may be NULL) takes 1 where a length exceeds the page table or a position the rope
+ * tables, 3 where a page id lies outside the cache. A bad length is cut to what the table holds; a
+ * bad page reads as zeros and is not written; a bad position writes nothing.
+ */
+typedef struct mt_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  const void* page_table;
+  const void* kv_lens;
+  long long k_page_stride, k_head_stride, k_row_stride;
+  long long v_page_stride, v_head_stride, v_row_stride;
+  long long table_stride;
+  int pages, heads, page_size, head_dim, max_pages, batch, type;
+} mt_paged_kv;
+
+/*
+ * Head RMSNorm + rotate-half RoPE of packed new tokens, the query rows to q_out [tokens][nq][D] and
+ * the key and value rows into their pages: qkv [tokens] rows of (nq + 2 heads) * D, qkv_row elements
+ * apart. Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1])
+ * and its last kv_lens[b] positions; cu_seqlens NULL: one token per sequence. Rows behind the last
+ * sequence are left alone. q_norm / k_norm [D]; cos_tab / sin_tab [table_rows][D] in the cache's type,
+ * or fp32 with table_fp32. All arithmetic is fp32 with one rounding at the store (mt_qk_rope_kv rounds
+ * after every step, as the reference does). A page that is written belongs to one sequence.
+ */
+int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_norm, const void* cos_tab,
+                     const void* sin_tab, int table_rows, int table_fp32, const mt_paged_kv* kv,
+                     const void* cu_seqlens, int tokens, int nq, int qkv_row, void* q_out, float eps,
+                     void* status, int flags, void* stream);
+
+/*
+ * Attention of one new token per sequence over its pages: out [batch][nq][D] =
+ * softmax(scale q k^T) v over keys 0 .. kv_lens[b] - 1; q [batch] rows q_row elements apart, heads
+ * q_head apart; query head h reads key head h / (nq / heads), nq / heads <= 64. A sequence of length 0
+ * gives zeros.
+ */
+int mt_paged_attention_decode(const void* q, int q_row, int q_head, const mt_paged_kv* kv, int nq, float scale,
+                              void* out, void* status, int flags, void* stream);
+
+/*
+ * Attention of packed prompts: q [tokens_q], k and v [tokens_k] rows with their row and head strides
+ * in elements; sequence b holds query rows cu_q[b] .. cu_q[b + 1] - 1 and key rows cu_k[b] ..
+ * cu_k[b + 1] - 1 (int32 [batch + 1]). The last query stands at the last key: with causal != 0, query
+ * i of n sees keys 0 .. len - n + i, which for len < n leaves the first rows without a key (zeros).
+ * out [tokens_q][nq][D]; rows outside every sequence are left as they were.
+ */
+int mt_packed_attention(const void* q, int q_row, int q_head, const void* k, int k_row, int k_head, const void* v,
+                        int v_row, int v_head, const void* cu_q, const void* cu_k, int batch, int tokens_q,
+                        int tokens_k, int nq, int nkv, int head_dim, int type, int causal, float scale, void* out,
+                        int flags, void* stream);
+
+/* mt_packed_attention, causal, of the newest cu_seqlens[b + 1] - cu_seqlens[b] tokens over pages. */
+int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const mt_paged_kv* kv, const void* cu_seqlens,
+                              int tokens, int nq, float scale, void* out, void* status, int flags, void* stream);
+
+/*
  * Output heads of one decode step with greedy selection: final add_rmsnorm of
  * (x + residual), logits of the n_text text-head rows and n_cb audio codebooks of `vocab`
  * rows each, argmax with the first-index tie rule, delay-pattern masks, next token ids

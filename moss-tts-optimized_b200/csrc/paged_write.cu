@@ -1,0 +1,148 @@
+// Write of new tokens into a paged key-value cache (sm_100a): per head RMSNorm, rotate-half rotary
+// position, the query rows out and the key and value rows into their pages, for packed tokens of
+// sequences of different lengths.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w        r_i = y_i cos_i -+ y_(i +- D/2) sin_i
+//
+// Everything between the 16-bit input and output is fp32 and rounds once, at the store.
+#include "paged.cuh"
+
+namespace mt {
+namespace paged {
+
+struct WriteArgs {
+  const char* qkv;      // [tokens][(nq + 2 nkv) D], rows qkv_row elements apart
+  const char *qw, *kw;  // [D]
+  const char *cos_tab, *sin_tab;  // [table_rows][D]
+  const int* cu;        // [batch + 1], or null: token t is sequence t's only one
+  char* q_out;          // [tokens][nq][D]
+  int* status;
+  long long qkv_row;
+  int tokens, nq, table_rows;
+  float eps;
+};
+
+constexpr int kThreads = 128;
+
+// Bound by HBM. One CTA a token: D/8 lanes hold one head (16 bytes each), so the mean of squares is
+// a shuffle inside the group and the rotation's partner element, D/2 away, is in the lane
+// (D/8)/2 away.
+template <typename T, typename Tab, int D>
+__global__ void __launch_bounds__(kThreads) qk_rope_paged(WriteArgs a, Pages p) {
+  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
+  const int t = blockIdx.x, lane = threadIdx.x & 31;
+  const int group = threadIdx.x / kLanes, sub = threadIdx.x % kLanes;
+  pdl_wait();
+  pdl_trigger();
+  const int b = a.cu ? sequence_of(a.cu, p.batch, t, lane) : t;
+  if (b >= p.batch || (a.cu && a.cu[b] > t)) return;  // behind the last sequence
+  const int len = p.lens[b];
+  const int pos = a.cu ? len - a.cu[b + 1] + t : len - 1;
+  if (pos < 0 || pos >= a.table_rows || (pos >> p.shift) >= p.max_pages) {
+    if (a.status && threadIdx.x == 0) atomicExch(a.status, kStatusPosition);
+    return;
+  }
+  const int page = page_of(p, p.table + (long long)b * p.table_row, pos, threadIdx.x == 0 ? a.status : nullptr);
+  const int slot = pos & ((1 << p.shift) - 1);
+
+  float c[8], s[8];
+  if constexpr (sizeof(Tab) == 4) {
+    const float4* cp = reinterpret_cast<const float4*>(a.cos_tab + ((long long)pos * D + sub * 8) * 4);
+    const float4* sp = reinterpret_cast<const float4*>(a.sin_tab + ((long long)pos * D + sub * 8) * 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 cv = cp[i], sv = sp[i];
+      c[4 * i] = cv.x, c[4 * i + 1] = cv.y, c[4 * i + 2] = cv.z, c[4 * i + 3] = cv.w;
+      s[4 * i] = sv.x, s[4 * i + 1] = sv.y, s[4 * i + 2] = sv.z, s[4 * i + 3] = sv.w;
+    }
+  } else {
+    const uint4 cv = *reinterpret_cast<const uint4*>(a.cos_tab + ((long long)pos * D + sub * 8) * 2);
+    const uint4 sv = *reinterpret_cast<const uint4*>(a.sin_tab + ((long long)pos * D + sub * 8) * 2);
+    const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 cf = Elem<T>::unpack(cw[i]), sf = Elem<T>::unpack(sw[i]);
+      c[2 * i] = cf.x, c[2 * i + 1] = cf.y, s[2 * i] = sf.x, s[2 * i + 1] = sf.y;
+    }
+  }
+  const float sign = sub < kLanes / 2 ? -1.f : 1.f;
+  const int heads = a.nq + 2 * p.heads;
+  const char* src = a.qkv + (long long)t * a.qkv_row * 2;
+  // every lane takes part in the shuffles: heads past the last are computed on zeros and not stored
+  for (int h0 = 0; h0 < heads; h0 += kGroups) {
+    const int h = h0 + group;
+    const bool live = h < heads;
+    const uint4 v = live ? *reinterpret_cast<const uint4*>(src + ((long long)h * D + sub * 8) * 2) : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float x[8], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<T>::unpack(w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+    const uint4 nv = *reinterpret_cast<const uint4*>((h < a.nq ? a.qw : a.kw) + sub * 16);
+    const uint32_t nw[4] = {nv.x, nv.y, nv.z, nv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Elem<T>::unpack(nw[i]);
+      x[2 * i] *= inv * f.x;
+      x[2 * i + 1] *= inv * f.y;
+    }
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = __shfl_xor_sync(0xffffffffu, x[2 * i], kLanes / 2);
+      const float p1 = __shfl_xor_sync(0xffffffffu, x[2 * i + 1], kLanes / 2);
+      r[i] = Elem<T>::pack(fmaf(x[2 * i], c[2 * i], sign * p0 * s[2 * i]),
+                           fmaf(x[2 * i + 1], c[2 * i + 1], sign * p1 * s[2 * i + 1]));
+    }
+    if (!live) continue;
+    const uint4 out = make_uint4(r[0], r[1], r[2], r[3]);
+    if (h < a.nq)
+      *reinterpret_cast<uint4*>(a.q_out + (((long long)t * a.nq + h) * D + sub * 8) * 2) = out;
+    else if (page >= 0 && h < a.nq + p.heads)
+      *reinterpret_cast<uint4*>(p.k + (page * p.k_page + (h - a.nq) * p.k_head + slot * p.k_row + sub * 8) * 2) = out;
+    else if (page >= 0)  // values as they are
+      *reinterpret_cast<uint4*>(p.v + (page * p.v_page + (h - a.nq - p.heads) * p.v_head + slot * p.v_row + sub * 8) * 2) = v;
+  }
+}
+
+template <typename T, typename Tab>
+static cudaError_t launch_write(const WriteArgs& a, const Pages& p, int d, cudaStream_t s, int flags) {
+  return d == 128 ? launch(qk_rope_paged<T, Tab, 128>, dim3(a.tokens), dim3(kThreads), 0, s, flags, a, p)
+                  : launch(qk_rope_paged<T, Tab, 64>, dim3(a.tokens), dim3(kThreads), 0, s, flags, a, p);
+}
+
+}  // namespace paged
+}  // namespace mt
+
+using namespace mt;
+
+// Head norm, rotary position and page write of packed new tokens (see the header).
+MT_API int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_norm, const void* cos_tab,
+                            const void* sin_tab, int table_rows, int table_fp32, const mt_paged_kv* kv,
+                            const void* cu_seqlens, int tokens, int nq, int qkv_row, void* q_out, float eps,
+                            void* status, int flags, void* stream) {
+  paged::Pages p;
+  if (!qkv || !q_norm || !k_norm || !cos_tab || !sin_tab || !q_out || !paged::pages_of(kv, &p)) return kBadArgument;
+  if (table_rows < 1 || tokens < 1 || nq < 1 || qkv_row % 8 || (!cu_seqlens && tokens != kv->batch))
+    return kBadArgument;
+  if (qkv_row < (long long)(nq + 2LL * kv->heads) * kv->head_dim) return kBadArgument;
+  const void* wide[6] = {qkv, q_norm, k_norm, cos_tab, sin_tab, q_out};
+  for (const void* x : wide)
+    if (!aligned(x, 16)) return kBadArgument;
+  const paged::WriteArgs a{(const char*)qkv,     (const char*)q_norm, (const char*)k_norm, (const char*)cos_tab,
+                           (const char*)sin_tab, (const int*)cu_seqlens, (char*)q_out,   (int*)status,
+                           qkv_row,              tokens,              nq,                  table_rows,
+                           eps};
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (kv->type == 0)
+    return table_fp32 ? paged::launch_write<__nv_bfloat16, float>(a, p, kv->head_dim, s, flags)
+                      : paged::launch_write<__nv_bfloat16, __nv_bfloat16>(a, p, kv->head_dim, s, flags);
+  return table_fp32 ? paged::launch_write<__half, float>(a, p, kv->head_dim, s, flags)
+                    : paged::launch_write<__half, __half>(a, p, kv->head_dim, s, flags);
+}

@@ -161,3 +161,231 @@ def qk_rope_decode(qkv, q_weight, k_weight, cos, sin, cache, layer_idx, position
                 scratch.tickets.data_ptr(), 1, nq, nkv, length, scratch.splits, float(eps), None, 0,
                 native.stream_of(qkv))
     return out
+
+
+# ---------------------------------------------------------------------------- paged key-value cache
+_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _heads3(name, t, dtype, dev):
+    """Row and head stride of ``t`` ``[rows, heads, D]``, whose D elements are adjacent."""
+    if t.ndim != 3 or t.dtype != dtype or t.device != dev:
+        raise ValueError(f"{name} must be [rows, heads, D], of the queries' type and device")
+    rows, heads, d = t.shape
+    row, head, one = t.stride()
+    if rows <= 1:  # the stride of a dimension of one says nothing
+        row = heads * d
+    if heads <= 1:
+        head = d
+    if one != 1 or row % 8 or head % 8 or not 0 < row < 1 << 31 or not 0 < head < 1 << 31 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: D must be adjacent, rows and heads 16-byte aligned and not broadcast")
+    return row, head
+
+
+def _query(q, heads, d):
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise ValueError("CUDA tensors required (there is no CPU path)")
+    if q.dtype not in _TYPES:
+        raise ValueError("bf16 or fp16 tensors required")
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise ValueError("This attention has no backward pass")
+    row, head = _heads3("q", q, q.dtype, q.device)
+    nq = q.shape[1]
+    if q.shape[2] != d or d not in (64, 128):
+        raise ValueError("head_dim must be 64 or 128, the same for queries and keys")
+    if nq == 0 or heads == 0 or nq % heads or nq // heads > 64:
+        raise ValueError("Query heads must be 1 to 64 times the key heads")
+    return row, head
+
+
+def _ints(name, t, n, dev):
+    """An int32 vector of ``n`` elements (lengths or offsets)."""
+    if t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] != n or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector of {n} elements on the queries' device")
+    return t.data_ptr()
+
+
+def _status(status, dev):
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() != 1 or status.device != dev:
+        raise ValueError("status must be a one-element int32 tensor on the queries' device")
+    return status.data_ptr()
+
+
+def _out(out, shape, like):
+    if out is None:
+        return torch.empty(shape, device=like.device, dtype=like.dtype)
+    if out.shape != shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous {like.dtype} tensor {tuple(shape)} on the queries' device")
+    return out
+
+
+def _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev):
+    """``mt_paged_kv`` of one layer's pages, as bytes."""
+    if k_pages.ndim != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages must be [pages, heads, page_size, D]")
+    pages, heads, size, d = k_pages.shape
+    if size not in (16, 32, 64, 128, 256):
+        raise ValueError("page_size must be a power of two, 16 to 256")
+    if d not in (64, 128):
+        raise ValueError("head_dim must be 64 or 128, the same for queries and keys")
+    if pages < 1 or pages >= 1 << 31 or heads < 1:
+        raise ValueError("The cache has no pages")
+    strides = []
+    for t in (k_pages, v_pages):
+        if t.dtype != dtype or t.device != dev:
+            raise ValueError("The pages must have the queries' type and device")
+        page, head, row, one = t.stride()
+        if pages == 1:  # the stride of a dimension of one says nothing
+            page = heads * size * d
+        if heads == 1:
+            head = size * d
+        if one != 1 or page % 8 or head % 8 or row % 8 or min(page, head, row) <= 0 or t.data_ptr() % 16:
+            raise ValueError("pages: D must be adjacent, pages, heads and rows 16-byte aligned and not broadcast")
+        strides += (page, head, row)
+    if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.device != dev:
+        raise ValueError("page_table must be int32 [batch, max_pages] on the queries' device")
+    batch, most = page_table.shape
+    if batch < 1 or most < 1 or most * size > 1 << 30 or page_table.stride(1) != 1:
+        raise ValueError("page_table must have rows of 1 or more adjacent entries, for up to 2^30 tokens")
+    return native.PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+                                _ints("kv_lens", kv_lens, batch, dev), *strides, page_table.stride(0),
+                                pages, heads, size, d, most, batch, _TYPES[dtype])
+
+
+def _call_on(dev, name, *args):
+    """``native.call`` on the tensors' device and its current stream."""
+    if torch.cuda.current_device() == dev.index:
+        native.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            native.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, kv_lens, cu_seqlens, eps, *,
+                  out=None, status=None):
+    """QK-norm + RoPE of packed new tokens and their write into a paged key-value cache.
+
+    ``qkv`` ``[tokens, (nq + 2 nkv) * D]`` (bf16 or fp16, rows may be strided); ``cos`` / ``sin`` the RoPE
+    tables ``[max_len, D]`` in that type or fp32. Key j of sequence b lies in row ``j % page_size`` of page
+    ``page_table[b, j // page_size]`` (int32 ``[batch, max_pages]``) of ``k_pages`` / ``v_pages``
+    ``[pages, nkv, page_size, D]`` (any strides with adjacent D; page_size a power of two, 16 to 256; D 64 or
+    128). ``kv_lens`` int32 ``[batch]`` counts each sequence's tokens with the new ones; ``cu_seqlens`` int32
+    ``[batch + 1]`` are the new tokens' offsets in ``qkv``, or None for one token per sequence. Returns the
+    rotated queries ``[tokens, nq, D]`` (in ``out`` if given); rows behind the last sequence are not written.
+
+    Unlike ``qk_rope_decode``, whose intermediate roundings are the reference's, this rounds once, at the
+    store. A page that is written must belong to one sequence. ``status`` (int32, one element) takes 1 for a
+    position outside the tables (nothing is written for it) and 3 for a page id outside the cache.
+    """
+    if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda:
+        raise ValueError("CUDA tensors required (there is no CPU path)")
+    dev, dtype = qkv.device, qkv.dtype
+    if dtype not in _TYPES or qkv.ndim != 2 or qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) >= 1 << 31 \
+            or qkv.data_ptr() % 16:
+        raise ValueError("qkv must be bf16 or fp16 [tokens, (nq + 2 nkv) * D] with 16-byte aligned rows")
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        raise ValueError("This operator has no backward pass")
+    kv = _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev)
+    tokens, width = qkv.shape
+    nkv, d = k_pages.shape[1], k_pages.shape[3]
+    nq = width // d - 2 * nkv
+    if width % d or nq < 1 or (tokens > 1 and qkv.stride(0) < width):
+        raise ValueError("qkv must hold nq >= 1 query heads and the cache's key and value heads")
+    for w in (q_weight, k_weight):
+        if w.shape != (d,) or w.dtype != dtype or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
+            raise ValueError("q_weight and k_weight must be contiguous [D], of qkv's type and device")
+    if cos.ndim != 2 or cos.shape[1] != d or cos.shape[0] < 1 or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise ValueError("RoPE tables must be [max_len, D]")
+    for t in (cos, sin):
+        if t.dtype not in (dtype, torch.float32) or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError("RoPE tables must be contiguous, in qkv's type or fp32, on its device")
+    batch = page_table.shape[0]
+    if cu_seqlens is None and tokens != batch:
+        raise ValueError("Without cu_seqlens there is one token per sequence")
+    cu = None if cu_seqlens is None else _ints("cu_seqlens", cu_seqlens, batch + 1, dev)
+    st = _status(status, dev)
+    out = _out(out, (tokens, nq, d), qkv)
+    if tokens:
+        _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
+                 sin.data_ptr(), cos.shape[0], 1 if cos.dtype == torch.float32 else 0, kv, cu, tokens, nq,
+                 max(qkv.stride(0), width), out.data_ptr(), eps, st, 0)
+    return out
+
+
+def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=None, out=None, status=None):
+    """Attention of one new token per sequence over a paged key-value cache (``qk_rope_paged``'s).
+
+    ``q`` ``[batch, nq, D]`` (bf16 or fp16; rows and heads may be strided); query head h reads key head
+    ``h // (nq / nkv)``. Returns ``softmax(scale q k^T) v`` over keys ``0 .. kv_lens[b] - 1``, ``[batch, nq, D]``
+    (in ``out`` if given); ``scale`` defaults to ``1 / sqrt(D)``. A sequence of length 0 gives zeros.
+    ``status`` as in ``qk_rope_paged``: a length beyond the page table (1) is cut, a page id outside the
+    cache (3) reads as zeros.
+    """
+    row, head = _query(q, k_pages.shape[1], k_pages.shape[-1])
+    dev = q.device
+    kv = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
+    batch, nq, d = q.shape
+    if page_table.shape[0] != batch:
+        raise ValueError("page_table must have a row for each query row")
+    st = _status(status, dev)
+    out = _out(out, (batch, nq, d), q)
+    _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
+             out.data_ptr(), st, 0)
+    return out
+
+
+def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, scale=None, out=None):
+    """Attention of packed sequences of different lengths, causal or over all of a sequence's keys.
+
+    ``q`` ``[tokens, nq, D]``, ``k`` and ``v`` ``[tokens_k, nkv, D]`` (bf16 or fp16, D 64 or 128; rows and heads
+    may be strided, so slices of one ``q | k | v`` projection do); ``cu_seqlens_q`` / ``cu_seqlens_k`` int32
+    ``[batch + 1]`` row offsets, the second None where they are the same. The last query of a sequence stands
+    at its last key: with ``causal``, query i of n sees keys ``0 .. len - n + i``; a query without a key gives
+    zeros. Returns ``[tokens, nq, D]`` (in ``out`` if given); rows outside every sequence are not written.
+    """
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError("k and v must be [tokens, nkv, D]")
+    row, head = _query(q, k.shape[1], k.shape[2])
+    dev = q.device
+    k_row, k_head = _heads3("k", k, q.dtype, dev)
+    v_row, v_head = _heads3("v", v, q.dtype, dev)
+    tokens, nq, d = q.shape
+    batch = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.ndim == 1 else 0
+    if batch < 1:
+        raise ValueError("cu_seqlens_q must hold batch + 1 offsets of 1 or more sequences")
+    cu_q = _ints("cu_seqlens_q", cu_seqlens_q, batch + 1, dev)
+    cu_k = cu_q if cu_seqlens_k is None else _ints("cu_seqlens_k", cu_seqlens_k, batch + 1, dev)
+    out = _out(out, (tokens, nq, d), q)
+    if tokens == 0:
+        return out
+    if k.shape[0] == 0:  # no key anywhere: every row of a sequence is zero, as the kernel would leave it
+        k, v, k_row, k_head, v_row, v_head = q, q, row, head, row, head
+        cu_k = torch.zeros(batch + 1, device=dev, dtype=torch.int32).data_ptr()
+    _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+             v_head, cu_q, cu_k, batch, tokens, max(1, k.shape[0]), nq, k.shape[1], d, _TYPES[q.dtype],
+             1 if causal else 0, d ** -0.5 if scale is None else scale, out.data_ptr(), 0)
+    return out
+
+
+def paged_attention_prompt(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens, *, scale=None, out=None, status=None):
+    """Causal attention of packed prompts, or chunks of them, over a paged key-value cache.
+
+    ``q`` ``[tokens, nq, D]`` are the newest tokens of every sequence, rows ``cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1`` (int32 ``[batch + 1]``) of the last ``kv_lens[b]`` positions; their keys and values
+    are in the pages already (``qk_rope_paged``). Query i of n sees keys ``0 .. kv_lens[b] - n + i``. Otherwise
+    as ``packed_attention``, with ``paged_attention_decode``'s cache and ``status``.
+    """
+    row, head = _query(q, k_pages.shape[1], k_pages.shape[-1])
+    dev = q.device
+    kv = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
+    tokens, nq, d = q.shape
+    cu = _ints("cu_seqlens", cu_seqlens, page_table.shape[0] + 1, dev)
+    st = _status(status, dev)
+    out = _out(out, (tokens, nq, d), q)
+    if tokens:
+        _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
+                 d ** -0.5 if scale is None else scale, out.data_ptr(), st, 0)
+    return out

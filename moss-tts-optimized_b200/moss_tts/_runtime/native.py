@@ -8,6 +8,7 @@ does (``src/moss_tts/_runtime/attention_native.py:41-44``).
 """
 import ctypes
 import functools
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).with_name("libmoss_tts_b200.so")
@@ -52,6 +53,10 @@ SIGNATURES = {
     "mt_decode_layers": ([_P, _I, _I, _I, _P, _P, _P, _P, _I, _F, _P, _P, _P, _P, _I, _P], _I),
     "mt_prefill_qk_rope_kv": ([_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P], _I),
     "mt_prefill_attention": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
+    "mt_qk_rope_paged": ([_P] * 5 + [_I, _I, _P, _P, _I, _I, _I, _P, _F, _P, _I, _P], _I),
+    "mt_paged_attention_decode": ([_P, _I, _I, _P, _I, _F, _P, _P, _I, _P], _I),
+    "mt_packed_attention": ([_P, _I, _I] * 3 + [_P, _P] + [_I] * 8 + [_F, _P, _I, _P], _I),
+    "mt_paged_attention_prompt": ([_P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _I, _P], _I),
     "mt_heads_greedy": ([_P, _P, _P, _F] + [_P] * 11 + [_I] * 11 + [_P], _I),
 }
 
@@ -70,6 +75,11 @@ class DecodeLayer(ctypes.Structure):
     """``mt_decode_layer`` of include/moss_tts_b200.h."""
     _fields_ = [(name, ctypes.c_void_p) for name in ("qkv", "out", "gate_up", "down", "input_norm", "post_norm",
                                                      "q_norm", "k_norm", "k_cache", "v_cache")]
+
+
+# ``mt_paged_kv`` of include/moss_tts_b200.h, in its field order (packed to bytes: half the time of a
+# ctypes structure in a call whose kernel takes a few microseconds)
+PAGED_KV = struct.Struct("@4P7q7i4x")
 
 
 class NativeLibraryError(RuntimeError):
