@@ -1,11 +1,44 @@
 // Attention of packed prompts of different lengths (sm_100a), keys and values packed or in pages.
+//
+// For query row t of a sequence with n new tokens and len keys, at position len - n + t:
+//   s_j = scale q k_j over the keys it sees, p_j = 2^((s_j - m) log2 e), o = sum p_j v_j / sum p_j
+// in one pass over tiles of 128 keys with a running reference m and sum per row.
+//
+// A work item is one key head and two query tiles of 128 rows: the rep = nq / nkv query heads of
+// 128 / rep tokens ride side by side in a tile (row = token * rep + head), so the group's heads share
+// every K and V tile and the causal edge cuts off 128 / rep tokens at a time, not 128. Warps of a CTA:
+//   0-3, 4-7  softmax of query tile 0 and 1, one thread a row
+//   8         issues the tcgen05.mma: S_i = Q_i K^T (both in shared memory) and O_i += P_i V (P in TMEM)
+//   9         loads Q, and K and V tiles through a ring, by TMA with the 128-byte swizzle
+//   10, 11    fill up the third warpgroup, whose registers go to the softmax warps
+// TMEM: S_0 | S_1 | O_0 | O_1; P_i overwrites S_i (16-bit, half its columns) once its row is in
+// registers. While one tile's softmax runs, the tensor core works for the other.
 #include "paged.cuh"
+#include "tensor_core.cuh"
 
 namespace mt {
 namespace prompt {
 
+using namespace tcore;
 using paged::Elem;
 using paged::Pages;
+using pipe::mbar_arrive;
+using pipe::mbar_expect_tx;
+using pipe::mbar_init;
+using pipe::mbar_try_wait;
+using pipe::mbar_try_wait_sleep;
+
+__device__ int g_prompt_error;  // set when a bounded wait expired (read through mt_read_error_word)
+
+constexpr int kTile = 128;      // query rows of a tile and keys of a step
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kThreads = 384;
+constexpr int kTmemCols = 512;
+// A row that needs the slow path (below) keeps its warp busy for long; far above that all the same.
+constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
+// The reference a row's exponentials are taken against follows the running maximum only when that
+// is 2^8 above it: weights up to 256 lose nothing in fp32 sums and 16-bit floating weights, and the
+// accumulator is rescaled once or twice a row instead of at every new maximum.
+constexpr float kSlack = 8.f;
 
 struct PromptArgs {
   const char* q;     // [tokens_q][nq][D]
@@ -14,7 +47,8 @@ struct PromptArgs {
   const int *cu_q, *cu_k;
   int* status;
   long long q_row, q_head, k_row, k_head, v_row, v_head;
-  int tokens_q, tokens_k, batch, nq, rep, causal;
+  int tokens_q, tokens_k, batch, nq, nkv, rep, causal;
+  int tok;           // tokens of a query tile: 128 / rep
   float scale;       // scale * log2 e
 };
 
@@ -25,36 +59,102 @@ __device__ __forceinline__ void span_of(const int* cu, int b, int tokens, int& f
   n = max(min(cu[b + 1], tokens) - first, 0);
 }
 
-// One warp a (token, query head).
+struct Item {
+  int b, kh, q0, lq, k0, len;  // sequence, key head, its rows
+  int t0;                      // first token of query tile 0
+  int n[2];                    // key tiles that query tile i reads
+};
+
+__device__ __forceinline__ int keys_seen(const PromptArgs& a, const Item& it, int t) {
+  return a.causal ? min(max(it.len - it.lq + t + 1, 0), it.len) : it.len;
+}
+
+// The items of a CTA in order. Flat item w = (query tile pair, key head), pairs in order of the
+// sequences and, inside one, from its end, where a causal row sees most. CTA c takes the c-th item of
+// even rounds of gridDim and the c-th from the end of odd ones: the costs fall along a sequence, and
+// this evens them out. Every warp walks the list by itself.
+struct Walk {
+  long round = 0;
+  int first = 0;    // 32 sequences from here on are scanned next
+  long before = 0;  // tile pairs of the sequences before `first`
+
+  template <bool PAGED>
+  __device__ bool next(const PromptArgs& a, const Pages& p, int lane, Item& it) {
+    const long g = gridDim.x;
+    const long w = round * g + ((round & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+    ++round;
+    const long pair = w / a.nkv;
+    it.kh = (int)(w - pair * a.nkv);
+    for (; first < a.batch; first += 32) {
+      int q0 = 0, lq = 0;
+      if (first + lane < a.batch) span_of(a.cu_q, first + lane, a.tokens_q, q0, lq);
+      const int count = (lq + 2 * a.tok - 1) / (2 * a.tok);
+      int upto = count;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + upto > pair);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        it.b = first + src;
+        it.q0 = __shfl_sync(0xffffffffu, q0, src);
+        it.lq = __shfl_sync(0xffffffffu, lq, src);
+        it.t0 = (int)(before + __shfl_sync(0xffffffffu, upto, src) - 1 - pair) * 2 * a.tok;
+        it.k0 = 0;
+        if (PAGED)
+          it.len = paged::clamped_len(p, it.b, lane == 0 ? a.status : nullptr);
+        else
+          span_of(a.cu_k, it.b, a.tokens_k, it.k0, it.len);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = it.t0 + i * a.tok;
+          it.n[i] = t < it.lq ? (keys_seen(a, it, min(t + a.tok, it.lq) - 1) + kTile - 1) / kTile : 0;
+        }
+        return true;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ bool wait_for(uint64_t* bar, unsigned parity, volatile int* dead) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  while (true) {
+    if (mbar_try_wait_sleep(bar, parity, 1000)) return true;
+    if (*dead) return false;
+    if (globaltimer_ns() - t0 > kDeadlineNs) {
+      *dead = 1;
+      return false;
+    }
+  }
+}
+// For copies and matrix products in flight when the kernel gives up: bounded, whatever `dead` says.
+__device__ __forceinline__ void drain(uint64_t* bar, unsigned parity) { (void)pipe::mbar_wait_bounded(bar, parity); }
+
+// A tile multiplies masked weights (zeros) with values too: a value row that is not finite makes
+// rows that must not see it NaN. A row that comes out non-finite is computed again, by one warp, from
+// its own keys alone, so that it holds what its keys say.
 template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(128) prompt_rows(PromptArgs a, Pages p) {
+__device__ __noinline__ void row_again(const PromptArgs* args, const Pages* pages, int b, int kh, int k0, int seen,
+                                       int row, int h) {
   constexpr int E = D / 32;
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (h >= a.nq) return;
-  const int b = paged::sequence_of(a.cu_q, a.batch, t, lane);
-  if (b >= a.batch) return;
-  int q0, nq_rows, k0 = 0, len;
-  span_of(a.cu_q, b, a.tokens_q, q0, nq_rows);
-  if (t < q0) return;
-  int* status = lane == 0 ? a.status : nullptr;
-  if (PAGED)
-    len = paged::clamped_len(p, b, status);
-  else
-    span_of(a.cu_k, b, a.tokens_k, k0, len);
-  const int keys = a.causal ? min(max(len - nq_rows + (t - q0) + 1, 0), len) : len;
-  const int kh = h / a.rep;
-  const uint32_t* qp = reinterpret_cast<const uint32_t*>(a.q + (t * a.q_row + h * a.q_head) * 2) + lane * (E / 2);
+  const PromptArgs& a = *args;
+  const Pages& p = *pages;
+  const int lane = threadIdx.x & 31;
+  const uint32_t* qp = reinterpret_cast<const uint32_t*>(a.q + (row * a.q_row + h * a.q_head) * 2) + lane * (E / 2);
   float q[E], o[E];
 #pragma unroll
   for (int e = 0; e < E / 2; ++e) {
     const float2 f = Elem<T>::unpack(qp[e]);
     q[2 * e] = f.x * a.scale, q[2 * e + 1] = f.y * a.scale;
   }
-  paged::row_attention<T, D>(q, keys, lane, [&](int j, const T*& k, const T*& v) {
+  paged::row_attention<T, D>(q, seen, lane, [&](int j, const T*& k, const T*& v) {
     if (PAGED) {
-      const long long page = paged::page_of(p, p.table + b * p.table_row, j, status);
+      const long long page = paged::page_of(p, p.table + b * p.table_row, j, nullptr);
       const int slot = j & ((1 << p.shift) - 1);
       k = page < 0 ? nullptr : (const T*)p.k + page * p.k_page + kh * p.k_head + slot * p.k_row;
       v = page < 0 ? nullptr : (const T*)p.v + page * p.v_page + kh * p.v_head + slot * p.v_row;
@@ -63,16 +163,394 @@ __global__ void __launch_bounds__(128) prompt_rows(PromptArgs a, Pages p) {
       v = (const T*)a.v + (k0 + j) * a.v_row + kh * a.v_head;
     }
   }, o);
-  uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)t * a.nq + h) * D * 2) + lane * (E / 2);
+  uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)row * a.nq + h) * D * 2) + lane * (E / 2);
 #pragma unroll
   for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e], o[2 * e + 1]);
 }
 
-template <typename T, bool PAGED>
-static cudaError_t launch_prompt(const PromptArgs& a, const Pages& p, int d, cudaStream_t s, int flags) {
-  const dim3 grid((unsigned)a.tokens_q, (unsigned)((a.nq + 3) / 4));
-  return d == 128 ? launch(prompt_rows<T, 128, PAGED>, grid, dim3(128), 0, s, flags, a, p)
-                  : launch(prompt_rows<T, 64, PAGED>, grid, dim3(128), 0, s, flags, a, p);
+template <int D>
+struct Layout {
+  static constexpr int kHalves = D / 64;                  // a tile is `halves` boxes of 64 elements a row
+  static constexpr uint32_t kBox = kTile * 128;           // bytes of a box
+  static constexpr uint32_t kTileBytes = kHalves * kBox;
+  static constexpr int kStages = D == 128 ? 5 : 10;       // ring of K and V tiles
+  static constexpr uint32_t kBytes = (2 + kStages) * kTileBytes + 1024;
+};
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_tiles(const __grid_constant__ PromptArgs a, const __grid_constant__ Pages p, const __grid_constant__ CUtensorMap qmap,
+                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using L = Layout<D>;
+  constexpr int NS = L::kStages;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free[2];
+  __shared__ __align__(8) uint64_t kv_full[NS], kv_empty[NS], drained;
+  __shared__ uint32_t tmem_s;
+  __shared__ int dead_s;
+  volatile int* dead = &dead_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;  // Q_0, Q_1, then the ring
+  const uint32_t ring = smem + 2 * L::kTileBytes;
+
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                 "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&q_full[i], 1);
+        mbar_init(&q_empty[i], 1);
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 4);  // a lane of each softmax warp
+        mbar_init(&o_full[i], 1);
+        mbar_init(&o_free[i], 4);
+      }
+      for (int i = 0; i < NS; ++i) {
+        mbar_init(&kv_full[i], 1);
+        mbar_init(&kv_empty[i], 1);
+      }
+      mbar_init(&drained, 1);
+      dead_s = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_s;
+  pdl_wait();
+  pdl_trigger();
+
+  // 168 registers a thread at launch: 2 x 216 for the softmax warpgroups, 72 for the third
+  if (warp < kMmaWarp)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  else
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  Walk walk;
+  Item it;
+  if (warp < kMmaWarp) {
+    // ------------------------------------------------------------------ softmax, one thread a row
+    const int i = warp >> 2, row = threadIdx.x & 127;
+    const int rtok = row / a.rep, rhead = row - rtok * a.rep;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes (lane << 16)
+    const uint32_t s_at = tmem + lanes + i * kTile, o_at = tmem + lanes + 2 * kTile + i * D;
+    unsigned steps = 0, items = 0;
+    // 2^(s k - m): a scale that is not positive is multiplied in first, so that the largest product
+    // belongs to the largest score
+    const bool plain = a.scale > 0.f;
+    const float k = plain ? a.scale : 1.f;
+    bool ok = true;
+    while (ok && walk.next<PAGED>(a, p, lane, it)) {
+      const int t = it.t0 + i * a.tok + rtok;  // this row's token
+      const bool live = rtok < a.tok && t < it.lq;
+      const int n = it.n[i], seen = live ? keys_seen(a, it, t) : 0;
+      // tiles that end before the first row's last key need no mask (rows without a token never count)
+      const int clear = n ? keys_seen(a, it, it.t0 + i * a.tok) / kTile : 0;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++steps) {
+        if (!(ok = wait_for(&s_full[i], steps & 1, dead))) break;
+        fence_after();
+        uint32_t sw[kTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, sw + 32 * c);
+        wait_ld();
+        hold<kTile>(sw);
+        float s[kTile];
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) s[c] = __uint_as_float(sw[c]);
+        if (!plain) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) s[c] *= a.scale;
+        }
+        if (j >= clear) {
+          const int left = seen - j * kTile;  // this row's keys from this tile's first on
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k;
+        const bool moves = mx - m > kSlack;  // the first tile too: m is -inf
+        if (__any_sync(0xffffffffu, moves)) {
+          const float to = moves ? mx : m;
+          const float f = moves ? ex2(m - to) : 1.f;
+          m = to;
+          l *= f;
+          if (j > 0) {  // S of this step is there, so the product of the last one is done
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t ow[32];
+              ld32(o_at + 32 * c, ow);
+              wait_ld();
+              hold<32>(ow);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
+              st32(o_at + 32 * c, ow);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const float2 k2 = make_float2(k, k), r2 = make_float2(-ref, -ref);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int x = 32 * c + 2 * e;
+            float2 v = fma2(make_float2(s[x], s[x + 1]), k2, r2);
+            v.x = ex2(v.x);
+            v.y = ex2(v.y);
+            sum[e & 1] = add2(sum[e & 1], v);
+            // the weights round to the values' type, as the tensor core wants them; the sum does not
+            pw[e] = Elem<T>::pack(v.x, v.y);
+          }
+          st16(s_at + 16 * c, pw);
+        }
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
+      }
+      if (!ok) break;
+      const int h = it.kh * a.rep + rhead;
+      uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2);
+      if (n == 0) {  // no key for any row of the tile
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+        }
+        continue;
+      }
+      if (!(ok = wait_for(&o_full[i], items++ & 1, dead))) break;
+      fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float odd = 0.f;  // not zero once an element is infinite or NaN
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t ow[32];
+        ld32(o_at + 32 * c, ow);
+        wait_ld();
+        hold<32>(ow);
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              f[x] = __uint_as_float(ow[8 * e + x]) * inv;
+              odd = fmaf(f[x], 0.f, odd);
+            }
+            dst[4 * c + e] = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]),
+                                        Elem<T>::pack(f[6], f[7]));
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[i]);
+      unsigned again = __ballot_sync(0xffffffffu, live && !(odd == 0.f));
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        row_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, __shfl_sync(0xffffffffu, seen, src),
+                               it.q0 + __shfl_sync(0xffffffffu, t, src), __shfl_sync(0xffffffffu, h, src));
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------------ tensor core
+    constexpr uint32_t kType = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
+    constexpr uint32_t kCommon = (1u << 4) | (kType << 7) | (kType << 10) | ((kTile >> 4) << 24);
+    constexpr uint32_t kScores = kCommon | ((kTile >> 3) << 17);              // K rows along K: as stored
+    constexpr uint32_t kValues = kCommon | (1u << 16) | ((D >> 3) << 17);     // V rows along N: transposed
+    unsigned loads = 0, steps[2] = {0, 0}, items[2] = {0, 0};
+    bool ok = true;
+    auto stage = [&](unsigned x) { return ring + (x % NS) * L::kTileBytes; };
+    auto landed = [&](unsigned x) { return wait_for(&kv_full[x % NS], (x / NS) & 1, dead); };
+    auto scores = [&](int i, uint32_t kt) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const uint32_t at = (d >> 2) * L::kBox + (d & 3) * 32;
+        mma_ss(tmem + i * kTile, operand(smem + i * L::kTileBytes + at, 16), operand(kt + at, 16), kScores, d > 0);
+      }
+      commit(&s_full[i]);
+    };
+    while (ok && walk.next<PAGED>(a, p, lane, it)) {
+      const int n = max(it.n[0], it.n[1]);
+      if (n == 0) continue;
+      const unsigned base = loads;
+      loads += 2 * n;
+      for (int i = 0; ok && i < 2; ++i)
+        if (it.n[i]) ok = wait_for(&q_full[i], items[i] & 1, dead);
+      if (!ok || !(ok = landed(base))) break;
+      if (elect_one()) {
+        for (int i = 0; i < 2; ++i)
+          if (it.n[i]) {
+            scores(i, stage(base));
+            if (it.n[i] == 1) commit(&q_empty[i]);
+          }
+        commit(&kv_empty[base % NS]);
+      }
+      __syncwarp();
+      for (int j = 0; ok && j < n; ++j) {
+        const unsigned vx = base + 2 * j + 1, kx = vx + 1;
+        bool v_here = false, k_here = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j >= it.n[i]) continue;
+          if (!v_here) {
+            if (!(ok = landed(vx))) break;
+            v_here = true;
+            const int rows = it.len - j * kTile;
+            if (rows < kTile) {
+              // what lies behind the last key is not this sequence's: zero, or its weight of zero
+              // would make NaN of a NaN
+              for (int x = rows * 8 + lane; x < kTile * 8; x += 32)
+#pragma unroll
+                for (int hf = 0; hf < L::kHalves; ++hf)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage(vx) + hf * L::kBox + x * 16), "r"(0)
+                               : "memory");
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+          }
+          if (!(ok = wait_for(&p_full[i], steps[i]++ & 1, dead))) break;
+          if (j == 0 && !(ok = wait_for(&o_free[i], (items[i]++ & 1) ^ 1, dead))) break;
+          const bool more = j + 1 < it.n[i];
+          if (more && !k_here) {
+            if (!(ok = landed(kx))) break;
+            k_here = true;
+          }
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int x = 0; x < kTile / 16; ++x)
+              mma_ts(tmem + 2 * kTile + i * D, tmem + i * kTile + 8 * x, operand(stage(vx) + x * 2048, L::kBox), kValues,
+                     j > 0 || x > 0);
+            if (more) {
+              scores(i, stage(kx));
+              if (j + 2 == it.n[i]) commit(&q_empty[i]);
+            } else {
+              commit(&o_full[i]);
+            }
+          }
+          __syncwarp();
+        }
+        if (ok && elect_one()) {
+          commit(&kv_empty[vx % NS]);
+          if (j + 1 < n) commit(&kv_empty[kx % NS]);
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) commit(&drained);  // before the TMEM is given back
+    __syncwarp();
+    drain(&drained, 0);
+  } else if (warp == kLoadWarp) {
+    // ------------------------------------------------------------------ loads
+    unsigned loads = 0, items[2] = {0, 0};
+    bool ok = true;
+    const int rows_q = a.tok * a.rep;
+    while (ok && walk.next<PAGED>(a, p, lane, it)) {
+      const int n = max(it.n[0], it.n[1]);
+      const int* table = PAGED ? p.table + it.b * p.table_row : nullptr;
+      for (int j = 0; ok && j < n; ++j) {
+        for (int kv = 0; kv < 2; ++kv, ++loads) {
+          if (j == 0) {  // Q_0, K, Q_1, V: in the order of their use
+            if (it.n[kv]) {
+              if (!(ok = wait_for(&q_empty[kv], (items[kv]++ & 1) ^ 1, dead))) break;
+              if (elect_one()) {
+                mbar_expect_tx(&q_full[kv], rows_q * 128 * L::kHalves);
+#pragma unroll
+                for (int hf = 0; hf < L::kHalves; ++hf)
+                  tma_3d(smem + kv * L::kTileBytes + hf * L::kBox, &qmap, hf * 64, it.kh * a.rep,
+                         it.q0 + it.t0 + kv * a.tok, &q_full[kv]);
+              }
+              __syncwarp();
+            }
+          }
+          const unsigned st = loads % NS;
+          if (!(ok = wait_for(&kv_empty[st], ((loads / NS) & 1) ^ 1, dead))) break;
+          const CUtensorMap* map = kv ? &vmap : &kmap;
+          const uint32_t dst = ring + st * L::kTileBytes;
+          if (PAGED) {
+            // one lane a box: the pages that hold keys of this tile, their halves
+            const int per = min(1 << p.shift, kTile), left = min(kTile, it.len - j * kTile);
+            const int boxes = (left + per - 1) / per;
+            if (lane == 0) mbar_expect_tx(&kv_full[st], boxes * per * 128 * L::kHalves);
+            __syncwarp();
+            if (lane < boxes * L::kHalves) {
+              const int box = lane / L::kHalves, hf = lane - box * L::kHalves, key = j * kTile + box * per;
+              int page = paged::page_of(p, table, key, a.status);
+              if (page < 0) page = p.pages;  // out of range: the box reads as zeros
+              tma_4d(dst + hf * L::kBox + box * per * 128, map, hf * 64, key & ((1 << p.shift) - 1), it.kh, page,
+                     &kv_full[st]);
+            }
+          } else if (elect_one()) {
+            mbar_expect_tx(&kv_full[st], L::kTileBytes);
+#pragma unroll
+            for (int hf = 0; hf < L::kHalves; ++hf)
+              tma_3d(dst + hf * L::kBox, map, hf * 64, it.kh, it.k0 + j * kTile, &kv_full[st]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (*dead) {  // copies in flight end before this CTA's shared memory does
+      for (unsigned x = loads > NS ? loads - NS : 0; x < loads; ++x) drain(&kv_full[x % NS], (x / NS) & 1);
+      for (int i = 0; i < 2; ++i)
+        if (items[i]) drain(&q_full[i], (items[i] - 1) & 1);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (dead_s && lane == 0) atomicExch(&g_prompt_error, 1);
+  }
+}
+
+// Query map: boxes of 64 elements x rep heads x 128 / rep tokens. Keys and values: 64 elements x up to
+// 128 rows of one head, of a page or of the packed rows.
+template <typename T, int D, bool PAGED>
+static cudaError_t launch_tiles(const PromptArgs& a, const Pages& p, cudaStream_t s, int flags) {
+  using L = Layout<D>;
+  constexpr bool fp16 = __is_same(T, __half);
+  CUtensorMap qm, km, vm;
+  const cuuint64_t qd[3] = {D, (cuuint64_t)a.nq, (cuuint64_t)a.tokens_q};
+  const cuuint64_t qs[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_row * 2};
+  const cuuint32_t qb[3] = {64, (cuuint32_t)a.rep, (cuuint32_t)a.tok};
+  bool ok = tensor_map(&qm, fp16, 3, a.q, qd, qs, qb);
+  if (PAGED) {
+    const cuuint64_t page = 1ull << p.shift;
+    const cuuint64_t d[4] = {D, page, (cuuint64_t)p.heads, (cuuint64_t)p.pages};
+    const cuuint64_t ks[3] = {(cuuint64_t)p.k_row * 2, (cuuint64_t)p.k_head * 2, (cuuint64_t)p.k_page * 2};
+    const cuuint64_t vs[3] = {(cuuint64_t)p.v_row * 2, (cuuint64_t)p.v_head * 2, (cuuint64_t)p.v_page * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(page < kTile ? page : kTile), 1, 1};
+    ok = ok && tensor_map(&km, fp16, 4, p.k, d, ks, box) && tensor_map(&vm, fp16, 4, p.v, d, vs, box);
+  } else {
+    const cuuint64_t d[3] = {D, (cuuint64_t)a.nkv, (cuuint64_t)a.tokens_k};
+    const cuuint64_t ks[2] = {(cuuint64_t)a.k_head * 2, (cuuint64_t)a.k_row * 2};
+    const cuuint64_t vs[2] = {(cuuint64_t)a.v_head * 2, (cuuint64_t)a.v_row * 2};
+    const cuuint32_t box[3] = {64, 1, kTile};
+    ok = ok && tensor_map(&km, fp16, 3, a.k, d, ks, box) && tensor_map(&vm, fp16, 3, a.v, d, vs, box);
+  }
+  if (!ok) return cudaErrorInvalidValue;
+  const long long most = ((long long)a.tokens_q / (2 * a.tok) + a.batch) * a.nkv;  // items at the most
+  const int ctas = (int)(most < sm_count() ? most : sm_count());
+  return launch(prompt_tiles<T, D, PAGED>, dim3(ctas), dim3(kThreads), L::kBytes, s, flags, a, p, qm, km, vm);
+}
+
+template <bool PAGED>
+static cudaError_t launch_prompt(const PromptArgs& a, const Pages& p, int d, int type, cudaStream_t s, int flags) {
+  if (type == 0)
+    return d == 128 ? launch_tiles<__nv_bfloat16, 128, PAGED>(a, p, s, flags)
+                    : launch_tiles<__nv_bfloat16, 64, PAGED>(a, p, s, flags);
+  return d == 128 ? launch_tiles<__half, 128, PAGED>(a, p, s, flags) : launch_tiles<__half, 64, PAGED>(a, p, s, flags);
 }
 
 static bool query_ok(const void* q, int q_row, int q_head, const void* cu, int tokens, int nq, int nkv, const void* out) {
@@ -81,6 +559,19 @@ static bool query_ok(const void* q, int q_row, int q_head, const void* cu, int t
 }
 
 }  // namespace prompt
+
+cudaError_t prompt_error_word(int* value, bool clear) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, prompt::g_prompt_error, sizeof(int));
+  if (e != cudaSuccess) return e;
+  *value |= v;
+  if (clear) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(prompt::g_prompt_error, &zero, sizeof(int));
+  }
+  return e;
+}
+
 }  // namespace mt
 
 using namespace mt;
@@ -95,13 +586,12 @@ MT_API int mt_packed_attention(const void* q, int q_row, int q_head, const void*
   if (k_row < 1 || k_head < 1 || v_row < 1 || v_head < 1 || k_row % 8 || k_head % 8 || v_row % 8 || v_head % 8 ||
       !aligned(k, 16) || !aligned(v, 16) || !aligned(cu_k, 4))
     return kBadArgument;
+  const int rep = nq / nkv;
   const prompt::PromptArgs a{(const char*)q, (const char*)k, (const char*)v, (char*)out, (const int*)cu_q,
                              (const int*)cu_k, nullptr, q_row, q_head, k_row, k_head, v_row, v_head,
-                             tokens_q, tokens_k, batch, nq, nq / nkv, causal != 0, scale * paged::kLog2e};
-  const paged::Pages none = {};
-  const cudaStream_t s = (cudaStream_t)stream;
-  return type == 0 ? prompt::launch_prompt<__nv_bfloat16, false>(a, none, head_dim, s, flags)
-                   : prompt::launch_prompt<__half, false>(a, none, head_dim, s, flags);
+                             tokens_q, tokens_k, batch, nq, nkv, rep, causal != 0, prompt::kTile / rep,
+                             scale * paged::kLog2e};
+  return prompt::launch_prompt<false>(a, paged::Pages{}, head_dim, type, (cudaStream_t)stream, flags);
 }
 
 // Causal attention of packed prompts over a paged cache (see the header).
@@ -110,10 +600,9 @@ MT_API int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const
   paged::Pages p;
   if (!paged::pages_of(kv, &p) || !prompt::query_ok(q, q_row, q_head, cu_seqlens, tokens, nq, kv->heads, out))
     return kBadArgument;
+  const int rep = nq / kv->heads;
   const prompt::PromptArgs a{(const char*)q, nullptr, nullptr, (char*)out, (const int*)cu_seqlens, nullptr, (int*)status,
-                             q_row, q_head, 0, 0, 0, 0, tokens, 0, kv->batch, nq, nq / kv->heads, 1,
-                             scale * paged::kLog2e};
-  const cudaStream_t s = (cudaStream_t)stream;
-  return kv->type == 0 ? prompt::launch_prompt<__nv_bfloat16, true>(a, p, kv->head_dim, s, flags)
-                       : prompt::launch_prompt<__half, true>(a, p, kv->head_dim, s, flags);
+                             q_row, q_head, 0, 0, 0, 0, tokens, 0, kv->batch, nq, kv->heads, rep, 1,
+                             prompt::kTile / rep, scale * paged::kLog2e};
+  return prompt::launch_prompt<true>(a, p, kv->head_dim, kv->type, (cudaStream_t)stream, flags);
 }
