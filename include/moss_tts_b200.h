@@ -397,10 +397,12 @@ int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_norm, co
  * Attention of one new token per sequence over its pages: out [batch][nq][D] =
  * softmax(scale q k^T) v over keys 0 .. kv_lens[b] - 1; q [batch] rows q_row elements apart, heads
  * q_head apart; query head h reads key head h / (nq / heads), nq / heads <= 64. A sequence of length 0
- * gives zeros.
+ * gives zeros. `workspace`: mt_paged_attention_decode_workspace bytes, 16-byte aligned, of any content; two
+ * calls that may run at once have one each.
  */
+int mt_paged_attention_decode_workspace(long long* bytes);
 int mt_paged_attention_decode(const void* q, int q_row, int q_head, const mt_paged_kv* kv, int nq, float scale,
-                              void* out, void* status, int flags, void* stream);
+                              void* out, void* workspace, void* status, int flags, void* stream);
 
 /*
  * Attention of packed prompts: q [tokens_q], k and v [tokens_k] rows with their row and head strides

@@ -1,64 +1,447 @@
 // Attention of one new token per sequence over a paged key-value cache (sm_100a).
+//
+//   s_j = scale q k_j,  p_j = 2^((s_j - m) log2 e),  o = sum p_j v_j / sum p_j      over all keys j
+//
+// Bound by HBM: every key and value row is read once, 4 D bytes for 4 D flops a query head. The work is
+// cut into chunks of 64 keys of one key head (and up to 8 of its query heads), laid out one after the
+// other over the sequences, and every CTA takes an equal run of chunks, wherever sequences begin and
+// end: a batch of ragged sequences and one long sequence both load all SMs alike. A run that covers
+// a sequence's head only in part leaves (m, l, o) in the workspace; a second kernel joins the parts,
+//   m = max m_i,  o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i,
+// in the order of the keys, so the same inputs give the same bits.
 #include "paged.cuh"
+#include "tensor_core.cuh"
 
 namespace mt {
 namespace paged {
 
+using namespace tcore;
+using pipe::mbar_arrive;
+using pipe::mbar_expect_tx;
+using pipe::mbar_init;
+using pipe::mbar_wait_bounded;
+
+__device__ int g_paged_error;  // set when a bounded wait expired (read through mt_read_error_word)
+
+constexpr int kChunk = 64;      // keys of a chunk
+constexpr int kHeads = 8;       // query heads of an item: rows 0-7 of the mma's 16 (8-15 take the
+                                // low halves of the weights)
+constexpr int kConsumers = 8;   // warps; groups of four take alternate chunks, 16 keys a warp
+constexpr int kDecodeThreads = (kConsumers + 1) * 32;
+
 struct DecodeArgs {
-  const char* q;  // [batch][nq][D]
-  char* out;      // [batch][nq][D], contiguous
+  const char* q;     // [batch][nq][D]
+  char* out;         // [batch][nq][D], contiguous
   int* status;
+  float* parts;      // [ctas][2][kHeads][D + 2]: o, m, l
+  int4* joins;       // [ctas]: {first output row, heads, parts, -}: the item that starts in this CTA
+                     // and ends in a later one; 0 parts where there is none
   long long q_row, q_head;
-  int nq, rep;
-  float scale;    // scale * log2 e
+  int nq, rep, groups;  // groups of up to 8 query heads of a key head
+  float scale;          // scale * log2 e
 };
 
-// One warp a query head.
+template <int D>
+struct Ring {
+  static constexpr int kHalves = D / 64;
+  static constexpr uint32_t kBox = kChunk * 128;  // 64 elements of a chunk's rows
+  static constexpr uint32_t kStage = 2 * kHalves * kBox;  // K and V
+  // an even number: a stage then belongs to one of the two groups of warps, which takes its phases
+  // one after the other (copies land out of order, and a parity tells only two phases apart)
+  static constexpr int kStages = D == 128 ? 6 : 12;
+  static constexpr uint32_t kMerge = kConsumers * kHeads * D * 4;
+  static constexpr uint32_t kBytes = kStages * kStage + kMerge + 1024;
+};
+
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  if constexpr (__is_same(T, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Byte offset of 16-byte piece `piece` of row r in a chunk: the 128-byte swizzle of its box.
+__device__ __forceinline__ uint32_t swizzled(int r, int piece) {
+  return (uint32_t)((piece >> 3) * (kChunk * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+}
+
+// Chunks of a sequence; one even where it is empty, so that its rows get their zeros.
+__device__ __forceinline__ int chunks_of(int len) { return len > kChunk ? (len + kChunk - 1) / kChunk : 1; }
+
+// An item in a CTA's run: chunks [c0, c1) of sequence b for key head kh, query heads of `group`.
+struct Run {
+  int b, kh, group, len, chunks, c0, c1;
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_decode_rows(DecodeArgs a, Pages p) {
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(kDecodeThreads, 1)
+    paged_decode(const __grid_constant__ DecodeArgs a, const __grid_constant__ Pages p,
+                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using R = Ring<D>;
+  constexpr int NS = R::kStages, NK = D / 16;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ long wsum[kConsumers + 1];
+  __shared__ float wm[kConsumers][kHeads], wl[kConsumers][kHeads];
+  __shared__ int dead_s;
+  volatile int* dead = &dead_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
+  float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp][head][D]
+  long* slab = reinterpret_cast<long*>(merge);  // chunks (of one head) of the sequences before thread t's slab
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    dead_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, b = blockIdx.y, h = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (h >= a.nq) return;
-  const int kh = h / a.rep, len = clamped_len(p, b, lane == 0 ? a.status : nullptr);
-  const int* row = p.table + b * p.table_row;
-  const uint32_t* qp = reinterpret_cast<const uint32_t*>(a.q + (b * a.q_row + h * a.q_head) * 2) + lane * (E / 2);
-  float q[E], o[E];
+  // prefix sums of the sequences' chunks: a slab of consecutive sequences a thread
+  const int per = (p.batch + kDecodeThreads - 1) / kDecodeThreads;
+  long mine = 0;
+  for (int b = tid * per; b < min((tid + 1) * per, p.batch); ++b)
+    mine += chunks_of(clamped_len(p, b, blockIdx.x == 0 ? a.status : nullptr));
+  long upto = mine;
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) {
-    const float2 f = Elem<T>::unpack(qp[e]);
-    q[2 * e] = f.x * a.scale, q[2 * e + 1] = f.y * a.scale;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
-  row_attention<T, D>(q, len, lane, [&](int j, const T*& k, const T*& v) {
-    const long long page = page_of(p, row, j, lane == 0 ? a.status : nullptr);
-    const int slot = j & ((1 << p.shift) - 1);
-    k = page < 0 ? nullptr : (const T*)p.k + page * p.k_page + kh * p.k_head + slot * p.k_row;
-    v = page < 0 ? nullptr : (const T*)p.v + page * p.v_page + kh * p.v_head + slot * p.v_row;
-  }, o);
-  uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.nq + h) * D * 2) + lane * (E / 2);
+  if (lane == 31) wsum[warp] = upto;
+  __syncthreads();
+  long total = 0;
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e], o[2 * e + 1]);
+  for (int w = 0; w <= kConsumers; ++w) {
+    if (w < warp) upto += wsum[w];
+    total += wsum[w];
+  }
+  slab[tid] = upto - mine;
+  __syncthreads();
+
+  const int per_seq = p.heads * a.groups;  // items of a sequence
+  const long work = total * per_seq;
+  // runs of equal length; no more of them than chunks, so that none between two others is empty
+  const long ctas = min((long)gridDim.x, work);
+  const long w0 = work * blockIdx.x / ctas, w1 = work * (blockIdx.x + 1) / ctas;
+  if (blockIdx.x >= ctas) {
+    if (tid == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // the sequence and item of chunk w0: every warp by itself
+  Run r;
+  long at = w0;  // the run's position in the flat order
+  {
+    int t = 0;  // the last slab that starts at or before w0 and holds something
+    for (int s = 0; s < kDecodeThreads; s += 32) {
+      const int n = __popc(__ballot_sync(0xffffffffu, slab[s + lane] * per_seq <= w0));
+      if (n) t = s + n - 1;
+      if (n < 32) break;
+    }
+    long before = slab[t] * per_seq;
+    int b = t * per;
+    while (true) {
+      r.len = clamped_len(p, b, nullptr);
+      r.chunks = chunks_of(r.len);
+      if (w0 < before + (long)r.chunks * per_seq) break;
+      before += (long)r.chunks * per_seq;
+      ++b;
+    }
+    r.b = b;
+    const long in = w0 - before;
+    const int item = (int)(in / r.chunks);
+    r.kh = item / a.groups;
+    r.group = item - r.kh * a.groups;
+    r.c0 = (int)(in - (long)item * r.chunks);
+    r.c1 = (int)min((long)r.chunks, r.c0 + (w1 - w0));
+  }
+  __syncthreads();  // `merge` takes the slabs' place
+  auto advance = [&]() {  // the next item, from its first chunk; false past the run's end
+    at += r.c1 - r.c0;
+    if (at >= w1) return false;
+    if (++r.group == a.groups) {
+      r.group = 0;
+      if (++r.kh == p.heads) {
+        r.kh = 0;
+        ++r.b;
+        r.len = clamped_len(p, r.b, nullptr);
+        r.chunks = chunks_of(r.len);
+      }
+    }
+    r.c0 = 0;
+    r.c1 = (int)min((long)r.chunks, w1 - at);
+    return true;
+  };
+
+  unsigned idx = 0;  // chunks of this CTA so far: stage idx % NS
+  if (warp == kConsumers) {
+    // -------------------------------------------------------------------- loads
+    bool ok = true;
+    const int rows = min(1 << p.shift, kChunk);  // of a box
+    do {
+      const int* table = p.table + r.b * p.table_row;
+      for (int c = r.c0; c < r.c1; ++c, ++idx) {
+        const unsigned st = idx % NS;
+        if (!(ok = !*dead && mbar_wait_bounded(&empty[st], ((idx / NS) & 1) ^ 1))) break;
+        const int left = min(kChunk, r.len - c * kChunk), boxes = (left + rows - 1) / rows;
+        if (lane == 0) mbar_expect_tx(&full[st], boxes * rows * 128 * 2 * R::kHalves);
+        __syncwarp();
+        // a lane a box: page, then half, then K or V
+        const int box = lane / (2 * R::kHalves), what = lane - box * 2 * R::kHalves;
+        if (box < boxes) {
+          const int key = c * kChunk + box * rows, hf = what % R::kHalves, v = what / R::kHalves;
+          int page = page_of(p, table, key, a.status);
+          if (page < 0) page = p.pages;  // out of range: the box reads as zeros
+          tma_4d(ring + st * R::kStage + what * R::kBox + box * rows * 128, v ? &vmap : &kmap, hf * 64,
+                 key & ((1 << p.shift) - 1), r.kh, page, &full[st]);
+        }
+        __syncwarp();
+      }
+    } while (ok && advance());
+    if (!ok) {
+      if (lane == 0) *dead = 1;
+      for (unsigned x = idx > NS ? idx - NS : 0; x < idx; ++x) mbar_wait_bounded(&full[x % NS], (x / NS) & 1);
+      if (lane == 0) atomicExch(&g_paged_error, 1);
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------------- attention
+  const int g = lane >> 2, t4 = lane & 3;  // this lane's query head, and its keys 2 t4 (+1) of 8
+  const int tok0 = 16 * (warp & 3), side = warp >> 2;
+  do {
+    const int heads = min(kHeads, a.rep - r.group * kHeads), row0 = r.b * a.nq + r.kh * a.rep + r.group * kHeads;
+    uint32_t qa[NK][2];
+    const char* qp = a.q + (r.b * a.q_row + (long long)(r.kh * a.rep + r.group * kHeads + g) * a.q_head) * 2;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      qa[kk][0] = g < heads ? *reinterpret_cast<const uint32_t*>(qp + 32 * kk + 4 * t4) : 0u;
+      qa[kk][1] = g < heads ? *reinterpret_cast<const uint32_t*>(qp + 32 * kk + 4 * t4 + 16) : 0u;
+    }
+    float o[2 * NK][4] = {};
+    float m = -INFINITY, l = 0.f;  // of head g; l over this lane's keys
+    for (int c = r.c0; c < r.c1; ++c, ++idx) {
+      if ((int)(idx & 1) != side) continue;
+      const unsigned st = idx % NS;
+      const int left = r.len - c * kChunk - tok0;  // keys of this warp's 16 and behind
+      const bool got = !*dead && mbar_wait_bounded(&full[st], (idx / NS) & 1);
+      if (!__all_sync(0xffffffffu, got)) {
+        if (lane == 0) *dead = 1, atomicExch(&g_paged_error, 1);
+      } else if (left > 0) {
+        const uint32_t kb = ring + st * R::kStage, vb = kb + R::kHalves * R::kBox;
+        if (left < 16) {
+          // rows past the last key are not the sequence's: zero, or their weight of zero would make
+          // NaN of a NaN
+          for (int x = lane; x < (16 - left) * 8 * R::kHalves; x += 32) {
+            const int hf = x / ((16 - left) * 8), rest = x - hf * (16 - left) * 8;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vb + hf * R::kBox + (tok0 + left) * 128 + rest * 16),
+                         "r"(0) : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next load
+          __syncwarp();
+        }
+        float s[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          uint32_t b[4];
+          ldsm(b, kb + swizzled(tok0 + (lane & 7) + 8 * (lane >> 4), 2 * kk + ((lane >> 3) & 1)));
+          mma16<T>(s[0], qa[kk][0], 0u, qa[kk][1], 0u, b[0], b[1]);
+          mma16<T>(s[1], qa[kk][0], 0u, qa[kk][1], 0u, b[2], b[3]);
+        }
+        float x[4], mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // keys 8 (e / 2) + 2 t4 + e % 2
+          x[e] = 8 * (e >> 1) + 2 * t4 + (e & 1) < left ? s[e >> 1][e & 1] * a.scale : -INFINITY;
+          mx = fmaxf(mx, x[e]);
+        }
+        // the reference follows the maximum when that is 2^8 above it (the sums are fp32)
+        if (__any_sync(0xffffffffu, mx - m > 8.f)) {
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float to = fmaxf(m, mx), f = to == -INFINITY ? 1.f : ex2(m - to);
+          m = to;
+          l *= f;
+#pragma unroll
+          for (int jd = 0; jd < 2 * NK; ++jd)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[jd][e] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int jn = 0; jn < 2; ++jn) {
+          const float p0 = ex2(x[2 * jn] - ref), p1 = ex2(x[2 * jn + 1] - ref);
+          l += p0 + p1;
+          // a weight as the sum of two 16-bit numbers, rows g and g + 8 of one product
+          hi[jn] = Elem<T>::pack(p0, p1);
+          const float2 h = Elem<T>::unpack(hi[jn]);
+          lo[jn] = Elem<T>::pack(p0 - h.x, p1 - h.y);
+        }
+#pragma unroll
+        for (int jp = 0; jp < NK; ++jp) {
+          uint32_t b[4];
+          ldsm_t(b, vb + swizzled(tok0 + (lane & 7) + 8 * ((lane >> 3) & 1), 2 * jp + (lane >> 4)));
+          mma16<T>(o[2 * jp], hi[0], lo[0], hi[1], lo[1], b[0], b[1]);
+          mma16<T>(o[2 * jp + 1], hi[0], lo[0], hi[1], lo[1], b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    // the eight warps' parts of the item, joined through shared memory
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t4 == 0) wm[warp][g] = m, wl[warp][g] = l;
+    float* mine_o = merge + (warp * kHeads + g) * D;
+#pragma unroll
+    for (int jd = 0; jd < 2 * NK; ++jd)
+      *reinterpret_cast<float2*>(mine_o + 8 * jd + 2 * t4) = make_float2(o[jd][0] + o[jd][2], o[jd][1] + o[jd][3]);
+    pipe::named_sync(1, kConsumers * 32);
+    const bool whole = r.c0 == 0 && r.c1 == r.chunks;
+    float* part = a.parts + ((long long)blockIdx.x * 2 + (r.c0 == 0 ? 1 : 0)) * kHeads * (D + 2);
+    for (int e = tid; e < heads * (D / 2); e += kConsumers * 32) {
+      const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kConsumers; ++w) mm = fmaxf(mm, wm[w][h]);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kConsumers; ++w) {
+        const float f = ex2(wm[w][h] - ref);
+        const float2 v = *reinterpret_cast<const float2*>(merge + (w * kHeads + h) * D + d);
+        ll = fmaf(f, wl[w][h], ll);
+        x0 = fmaf(f, v.x, x0);
+        x1 = fmaf(f, v.y, x1);
+      }
+      if (whole) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        *reinterpret_cast<uint32_t*>(a.out + ((long long)(row0 + h) * D + d) * 2) = Elem<T>::pack(x0 * inv, x1 * inv);
+      } else {
+        *reinterpret_cast<float2*>(part + h * D + d) = make_float2(x0, x1);
+        if (d == 0) part[kHeads * D + h] = mm, part[kHeads * D + kHeads + h] = ll;
+      }
+    }
+    if (tid == 0 && at + (r.c1 - r.c0) >= w1) {  // this CTA's last item: does it go on in the next ones?
+      int n = 0;
+      if (r.c0 == 0 && r.c1 < r.chunks) {
+        const long end = at + r.chunks;  // its end in the flat order
+        n = 2;
+        while (work * (blockIdx.x + n) / ctas < end) ++n;
+      }
+      a.joins[blockIdx.x] = make_int4(row0, heads, n, 0);
+    }
+    pipe::named_sync(1, kConsumers * 32);
+  } while (advance());
+}
+
+// Joins the parts of the items that more than one CTA worked on: block (c, h) the item that starts in
+// CTA c's run, query head h of its group.
+template <typename T, int D>
+__global__ void __launch_bounds__(D) paged_decode_join(const __grid_constant__ DecodeArgs a) {
+  pdl_wait();
+  const int c = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+  const int4 j = a.joins[c];
+  if (h >= j.y || j.z == 0) return;
+  auto part = [&](int i) {  // its first part in slot 1 of CTA c, the others in slot 0 of the next ones
+    return a.parts + ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * kHeads * (D + 2);
+  };
+  float m = -INFINITY;
+  for (int i = 0; i < j.z; ++i) m = fmaxf(m, part(i)[kHeads * D + h]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o = 0.f;
+  for (int i = 0; i < j.z; ++i) {
+    const float* x = part(i);
+    const float f = ex2(x[kHeads * D + h] - ref);
+    l = fmaf(f, x[kHeads * D + kHeads + h], l);
+    o = fmaf(f, x[h * D + d], o);
+  }
+  const float v = o * (l == 0.f ? 0.f : 1.f / l);
+  const uint32_t w = Elem<T>::pack(v, 0.f);
+  *reinterpret_cast<uint16_t*>(a.out + ((long long)(j.x + h) * D + d) * 2) = (uint16_t)w;
+}
+
+template <typename T, int D>
+static cudaError_t launch_decode(const DecodeArgs& a, const Pages& p, int ctas, cudaStream_t s, int flags) {
+  constexpr bool fp16 = __is_same(T, __half);
+  CUtensorMap km, vm;
+  const cuuint64_t page = 1ull << p.shift;
+  const cuuint64_t d[4] = {D, page, (cuuint64_t)p.heads, (cuuint64_t)p.pages};
+  const cuuint64_t ks[3] = {(cuuint64_t)p.k_row * 2, (cuuint64_t)p.k_head * 2, (cuuint64_t)p.k_page * 2};
+  const cuuint64_t vs[3] = {(cuuint64_t)p.v_row * 2, (cuuint64_t)p.v_head * 2, (cuuint64_t)p.v_page * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(page < kChunk ? page : kChunk), 1, 1};
+  if (!tensor_map(&km, fp16, 4, p.k, d, ks, box) || !tensor_map(&vm, fp16, 4, p.v, d, vs, box))
+    return cudaErrorInvalidValue;
+  cudaError_t e = launch(paged_decode<T, D>, dim3(ctas), dim3(kDecodeThreads), Ring<D>::kBytes, s, flags, a, p, km, vm);
+  if (e != cudaSuccess) return e;
+  return launch(paged_decode_join<T, D>, dim3(ctas, kHeads), dim3(D), 0, s, flags | kFlagPdl, a);
+}
+
+// CTAs of a call: one an SM, no more than there can be chunks.
+static int decode_ctas(int batch, int heads, int groups, long long max_len) {
+  const long long most = (long long)batch * heads * groups * ((max_len + kChunk - 1) / kChunk);
+  return (int)(most < sm_count() ? most : sm_count());
 }
 
 }  // namespace paged
+
+cudaError_t paged_error_word(int* value, bool clear) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, paged::g_paged_error, sizeof(int));
+  if (e != cudaSuccess) return e;
+  *value |= v;
+  if (clear) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(paged::g_paged_error, &zero, sizeof(int));
+  }
+  return e;
+}
+
 }  // namespace mt
 
 using namespace mt;
 
+// Workspace bytes of mt_paged_attention_decode on the current device, whatever the sizes.
+MT_API int mt_paged_attention_decode_workspace(long long* bytes) {
+  if (!bytes) return kBadArgument;
+  *bytes = (long long)sm_count() * (2 * paged::kHeads * (128 + 2) * sizeof(float) + sizeof(int4));
+  return 0;
+}
+
 // Decode attention over pages (see the header).
 MT_API int mt_paged_attention_decode(const void* q, int q_row, int q_head, const mt_paged_kv* kv, int nq, float scale,
-                                     void* out, void* status, int flags, void* stream) {
+                                     void* out, void* workspace, void* status, int flags, void* stream) {
   paged::Pages p;
-  if (!q || !out || !paged::pages_of(kv, &p) || nq < 1 || nq % kv->heads || nq / kv->heads > 64) return kBadArgument;
-  if (q_row < 1 || q_head < 1 || q_row % 8 || q_head % 8 || !aligned(q, 16) || !aligned(out, 16)) return kBadArgument;
-  const paged::DecodeArgs a{(const char*)q, (char*)out, (int*)status, q_row, q_head, nq, nq / kv->heads,
-                            scale * paged::kLog2e};
-  const dim3 grid((unsigned)((nq + 3) / 4), (unsigned)kv->batch);
-  if (kv->batch > 65535) return kBadArgument;
-  auto k = kv->type == 0 ? (kv->head_dim == 128 ? paged::paged_decode_rows<__nv_bfloat16, 128>
-                                                : paged::paged_decode_rows<__nv_bfloat16, 64>)
-                         : (kv->head_dim == 128 ? paged::paged_decode_rows<__half, 128>
-                                                : paged::paged_decode_rows<__half, 64>);
-  return launch(k, grid, dim3(128), 0, (cudaStream_t)stream, flags, a, p);
+  if (!q || !out || !workspace || !paged::pages_of(kv, &p) || nq < 1 || nq % kv->heads || nq / kv->heads > 64)
+    return kBadArgument;
+  if (q_row < 1 || q_head < 1 || q_row % 8 || q_head % 8 || !aligned(q, 16) || !aligned(out, 16) ||
+      !aligned(workspace, 16))
+    return kBadArgument;
+  const int rep = nq / kv->heads, groups = (rep + paged::kHeads - 1) / paged::kHeads;
+  const int ctas = paged::decode_ctas(kv->batch, kv->heads, groups, (long long)kv->max_pages * kv->page_size);
+  int4* joins = (int4*)workspace;
+  const paged::DecodeArgs a{(const char*)q, (char*)out, (int*)status, (float*)(joins + sm_count()), joins, q_row, q_head,
+                            nq, rep, groups, scale * paged::kLog2e};
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (kv->type == 0)
+    return kv->head_dim == 128 ? paged::launch_decode<__nv_bfloat16, 128>(a, p, ctas, s, flags)
+                               : paged::launch_decode<__nv_bfloat16, 64>(a, p, ctas, s, flags);
+  return kv->head_dim == 128 ? paged::launch_decode<__half, 128>(a, p, ctas, s, flags)
+                             : paged::launch_decode<__half, 64>(a, p, ctas, s, flags);
 }

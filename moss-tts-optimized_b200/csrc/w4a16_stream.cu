@@ -1025,6 +1025,7 @@ cudaError_t bf16_error_word(int* value, bool clear);
 cudaError_t gemm_error_word(int* value, bool clear);
 cudaError_t persist_error_word(int* value, bool clear);
 cudaError_t prompt_error_word(int* value, bool clear);
+cudaError_t paged_error_word(int* value, bool clear);
 }
 
 MT_API int mt_read_error_word(int* value, int clear) {
@@ -1039,5 +1040,6 @@ MT_API int mt_read_error_word(int* value, int clear) {
   if (e == cudaSuccess) e = gemm_error_word(value, clear != 0);
   if (e == cudaSuccess) e = persist_error_word(value, clear != 0);
   if (e == cudaSuccess) e = prompt_error_word(value, clear != 0);
+  if (e == cudaSuccess) e = paged_error_word(value, clear != 0);
   return (int)e;
 }

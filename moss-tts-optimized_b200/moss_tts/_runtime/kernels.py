@@ -264,6 +264,17 @@ def _call_on(dev, name, *args):
             native.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _workspace(size, dev):
+    """A workspace of ``size(device)`` bytes from torch's allocator, for one call: calls on other streams
+    and captured graphs have one each."""
+    if torch.cuda.current_device() == dev.index:
+        n = size(dev.index)
+    else:
+        with torch.cuda.device(dev):
+            n = size(dev.index)
+    return torch.empty(n, device=dev, dtype=torch.uint8)
+
+
 def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, kv_lens, cu_seqlens, eps, *,
                   out=None, status=None):
     """QK-norm + RoPE of packed new tokens and their write into a paged key-value cache.
@@ -332,8 +343,9 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
         raise ValueError("page_table must have a row for each query row")
     st = _status(status, dev)
     out = _out(out, (batch, nq, d), q)
+    ws = _workspace(native.paged_decode_workspace, dev)
     _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
-             out.data_ptr(), st, 0)
+             out.data_ptr(), ws.data_ptr(), st, 0)
     return out
 
 

@@ -54,7 +54,8 @@ SIGNATURES = {
     "mt_prefill_qk_rope_kv": ([_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P], _I),
     "mt_prefill_attention": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P], _I),
     "mt_qk_rope_paged": ([_P] * 5 + [_I, _I, _P, _P, _I, _I, _I, _P, _F, _P, _I, _P], _I),
-    "mt_paged_attention_decode": ([_P, _I, _I, _P, _I, _F, _P, _P, _I, _P], _I),
+    "mt_paged_attention_decode_workspace": ([_LLP], _I),
+    "mt_paged_attention_decode": ([_P, _I, _I, _P, _I, _F, _P, _P, _P, _I, _P], _I),
     "mt_packed_attention": ([_P, _I, _I] * 3 + [_P, _P] + [_I] * 8 + [_F, _P, _I, _P], _I),
     "mt_paged_attention_prompt": ([_P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _I, _P], _I),
     "mt_heads_greedy": ([_P, _P, _P, _F] + [_P] * 11 + [_I] * 11 + [_P], _I),
@@ -134,6 +135,14 @@ def decode_layers_workspace(n_layers: int, inter: int) -> int:
     """Workspace bytes of mt_decode_layers on the current device."""
     b = ctypes.c_longlong(0)
     call("mt_decode_layers_workspace", n_layers, inter, ctypes.byref(b))
+    return b.value
+
+
+@functools.cache
+def paged_decode_workspace(device: int) -> int:
+    """Workspace bytes of mt_paged_attention_decode on device ``device`` (the current one)."""
+    b = ctypes.c_longlong(0)
+    call("mt_paged_attention_decode_workspace", ctypes.byref(b))
     return b.value
 
 

@@ -386,6 +386,19 @@ def test_same_inputs_give_the_same_bits(cuda_device):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_long_context_many_calls_in_a_row(cuda_device):
+    """Dozens of chunks a CTA, calls queued without a wait between them: the chunks' copies land in any order."""
+    dev = cuda_device
+    kp, vp, table = make_cache(145, [32749], 8, 128, 128, BF, dev)
+    q, ln = normal(146, 1, 32, 128, device=dev), ints([32749], dev)
+    first = K.paged_attention_decode(q, kp, vp, table, ln)
+    outs = [K.paged_attention_decode(q, kp, vp, table, ln) for _ in range(200)]
+    assert all(torch.equal(first, x) for x in outs)
+    hk, hv = (opaged.gather(host(p), host(table)[0], 32749) for p in (kp, vp))
+    want, bound = oracle_rows(q, lambda b: (hk, hv), [0, 1], 128 ** -0.5, True, BF, DECODE_WEIGHT)
+    check("long context", first, want, bound)
+
+
 def test_empty_calls(cuda_device):
     dev = cuda_device
     z = torch.zeros(0, 4, 64, device=dev, dtype=BF)

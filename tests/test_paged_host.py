@@ -93,14 +93,15 @@ def test_entry_points_refuse_before_a_launch():
                                 dict(vs=(4096, -8, 64)), dict(pages=0), dict(heads=0), dict(size=8), dict(size=48),
                                 dict(size=512), dict(d=96), dict(most=0), dict(batch=0), dict(type=2), dict(lens=P + 2))]
     for x in bad_kv:
-        assert lib.mt_paged_attention_decode(P, 256, 64, x, 4, 0.1, P, None, 0, None) == 1
+        assert lib.mt_paged_attention_decode(P, 256, 64, x, 4, 0.1, P, P, None, 0, None) == 1
         assert lib.mt_paged_attention_prompt(P, 256, 64, x, P, 2, 4, 0.1, P, None, 0, None) == 1
         assert lib.mt_qk_rope_paged(P, P, P, P, P, 64, 0, x, P, 2, 4, 512, P, 1e-6, None, 0, None) == 1
     good = kv()
     for a in ((None, 256, 64, good, 4, 0.1, P), (P, 256, 64, good, 3, 0.1, P), (P, 256, 64, good, 0, 0.1, P),
               (P, 256, 64, good, 130, 0.1, P), (P, 250, 64, good, 4, 0.1, P), (P, 256, 64, good, 4, 0.1, P + 4),
               (P, 256, 64, None, 4, 0.1, P)):
-        assert lib.mt_paged_attention_decode(*a, None, 0, None) == 1
+        assert lib.mt_paged_attention_decode(*a, P, None, 0, None) == 1
+    assert lib.mt_paged_attention_decode(P, 256, 64, good, 4, 0.1, P, None, None, 0, None) == 1  # no workspace
     for a in ((P, 256, 64, P, 128, 64, P, 128, 64, P, P, 0), (P, 256, 64, P, 128, 60, P, 128, 64, P, P, 1),
               (P, 256, 64, P, 128, 64, P, 0, 64, P, P, 1), (P, 256, 64, P, 128, 64, P, 128, 64, None, P, 1)):
         assert lib.mt_packed_attention(*a, 4, 4, 4, 2, 64, 0, 1, 0.1, P, 0, None) == 1
