@@ -8,11 +8,16 @@
 // 128 / rep tokens ride side by side in a tile (row = token * rep + head), so the group's heads share
 // every K and V tile and the causal edge cuts off 128 / rep tokens at a time, not 128. Warps of a CTA:
 //   0-3, 4-7  softmax of query tile 0 and 1, one thread a row
-//   8         issues the tcgen05.mma: S_i = Q_i K^T (both in shared memory) and O_i += P_i V (P in TMEM)
+//   8         one thread issues the tcgen05.mma: S_i = Q_i K^T (both in shared memory) and
+//             O_i += P_i V (P in TMEM). A product of 128 x 128 x 16 is issued every ~66 cycles and runs
+//             for 64, so this thread does nothing else: its every wait shows in the tensor core
 //   9         loads Q, and K and V tiles through a ring, by TMA with the 128-byte swizzle
-//   10, 11    fill up the third warpgroup, whose registers go to the softmax warps
+//   10        zeroes the rows behind a sequence's last value
+//   11        fills up the third warpgroup, whose registers go to the softmax warps
 // TMEM: S_0 | S_1 | O_0 | O_1; P_i overwrites S_i (16-bit, half its columns) once its row is in
 // registers. While one tile's softmax runs, the tensor core works for the other.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "tensor_core.cuh"
 
@@ -26,19 +31,27 @@ using pipe::mbar_arrive;
 using pipe::mbar_expect_tx;
 using pipe::mbar_init;
 using pipe::mbar_try_wait;
-using pipe::mbar_try_wait_sleep;
 
 __device__ int g_prompt_error;  // set when a bounded wait expired (read through mt_read_error_word)
 
 constexpr int kTile = 128;      // query rows of a tile and keys of a step
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10, kThreads = 384;
 constexpr int kTmemCols = 512;
 // A row that needs the slow path (below) keeps its warp busy for long; far above that all the same.
 constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
-// The reference a row's exponentials are taken against follows the running maximum only when that
-// is 2^8 above it: weights up to 256 lose nothing in fp32 sums and 16-bit floating weights, and the
-// accumulator is rescaled once or twice a row instead of at every new maximum.
-constexpr float kSlack = 8.f;
+// The reference m that a row's exponentials are taken against is the largest score of its first tile,
+// and then moves only when it has to: weights far above 1 lose nothing in fp32 sums and 16-bit floating
+// weights, and an accumulator is rescaled once or twice a row instead of at every new maximum.
+// With bf16 weights, whose range is that of fp32, it moves when a step's weights add up to more than
+// kMost, for the next step: no maximum is looked for after the first tile. Scores that rise by 2^127
+// within one step leave an infinity, and the row is computed again (row_again). fp16 weights end at
+// 2^16: there the maximum is found in every step before the weights are, and m follows it when it is
+// 2^kSlack above.
+constexpr float kSlack = 8.f, kMost = 256.f;
+template <typename T>
+struct Reference {
+  static constexpr bool kExact = __is_same(T, __half);
+};
 
 struct PromptArgs {
   const char* q;     // [tokens_q][nq][D]
@@ -62,8 +75,12 @@ __device__ __forceinline__ void span_of(const int* cu, int b, int tokens, int& f
 struct Item {
   int b, kh, q0, lq, k0, len;  // sequence, key head, its rows
   int t0;                      // first token of query tile 0
-  int n[2];                    // key tiles that query tile i reads
+  int seen[2];                 // keys that query tile i's last row sees
 };
+// Key tiles of a query tile, and the keys that step j of them works on: 128, or 64 where the last
+// tile holds no more.
+__device__ __forceinline__ int tiles_of(int seen) { return (seen + kTile - 1) / kTile; }
+__device__ __forceinline__ bool half_step(int seen, int j) { return seen - j * kTile <= kTile / 2; }
 
 __device__ __forceinline__ int keys_seen(const PromptArgs& a, const Item& it, int t) {
   return a.causal ? min(max(it.len - it.lq + t + 1, 0), it.len) : it.len;
@@ -110,7 +127,7 @@ struct Walk {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = it.t0 + i * a.tok;
-          it.n[i] = t < it.lq ? (keys_seen(a, it, min(t + a.tok, it.lq) - 1) + kTile - 1) / kTile : 0;
+          it.seen[i] = t < it.lq ? keys_seen(a, it, min(t + a.tok, it.lq) - 1) : 0;
         }
         return true;
       }
@@ -120,15 +137,16 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ bool wait_for(uint64_t* bar, unsigned parity, volatile int* dead) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer_ns();
-  while (true) {
-    if (mbar_try_wait_sleep(bar, parity, 1000)) return true;
-    if (*dead) return false;
-    if (globaltimer_ns() - t0 > kDeadlineNs) {
-      *dead = 1;
-      return false;
+// Waits for a phase. Where that does not come, the kernel gives up: `dead` ends this and every later
+// wait at once, and the warps run through what is left of their work, to no use but within bounds.
+__device__ __forceinline__ void wait_for(uint64_t* bar, unsigned parity, volatile int* dead) {
+  unsigned long long t0 = 0;
+  for (unsigned tries = 0; !mbar_try_wait(bar, parity); ++tries) {
+    if (tries % 64 == 63 || *dead) {
+      if (*dead) return;
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kDeadlineNs) *dead = 1;
     }
   }
 }
@@ -184,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Layout<D>;
   constexpr int NS = L::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free[2];
-  __shared__ __align__(8) uint64_t kv_full[NS], kv_empty[NS], drained;
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_most[2], p_full[2], o_full[2], o_free[2];
+  __shared__ __align__(8) uint64_t kv_full[NS], kv_empty[NS], v_tail[NS], v_clean[NS], drained;
   __shared__ uint32_t tmem_s;
   __shared__ int dead_s;
   volatile int* dead = &dead_s;
@@ -202,13 +220,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&q_full[i], 1);
         mbar_init(&q_empty[i], 1);
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 4);  // a lane of each softmax warp
+        mbar_init(&p_most[i], 4);  // a lane of each softmax warp
+        mbar_init(&p_full[i], 4);
         mbar_init(&o_full[i], 1);
         mbar_init(&o_free[i], 4);
       }
       for (int i = 0; i < NS; ++i) {
         mbar_init(&kv_full[i], 1);
         mbar_init(&kv_empty[i], 1);
+        mbar_init(&v_tail[i], 1);
+        mbar_init(&v_clean[i], 1);
       }
       mbar_init(&drained, 1);
       dead_s = 0;
@@ -222,11 +243,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // 168 registers a thread at launch: 2 x 216 for the softmax warpgroups, 72 for the third
+  // 168 registers a thread at launch: 2 x 200 for the softmax warpgroups, 104 for the third
   if (warp < kMmaWarp)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
   else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   Walk walk;
   Item it;
   if (warp < kMmaWarp) {
@@ -240,42 +261,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     // belongs to the largest score
     const bool plain = a.scale > 0.f;
     const float k = plain ? a.scale : 1.f;
-    bool ok = true;
-    while (ok && walk.next<PAGED>(a, p, lane, it)) {
+    while (walk.next<PAGED>(a, p, lane, it)) {
       const int t = it.t0 + i * a.tok + rtok;  // this row's token
       const bool live = rtok < a.tok && t < it.lq;
-      const int n = it.n[i], seen = live ? keys_seen(a, it, t) : 0;
+      const int n = tiles_of(it.seen[i]), seen = live ? keys_seen(a, it, t) : 0;
       // tiles that end before the first row's last key need no mask (rows without a token never count)
       const int clear = n ? keys_seen(a, it, it.t0 + i * a.tok) / kTile : 0;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j, ++steps) {
-        if (!(ok = wait_for(&s_full[i], steps & 1, dead))) break;
-        fence_after();
-        uint32_t sw[kTile];
+      float last = 0.f;  // the sum of the last step's weights
+      // One step: a tile of scores to weights. COLS of its keys, MASKED where a row sees fewer.
+      auto step = [&](int j, auto cols, auto masked) {
+        constexpr int COLS = decltype(cols)::value, NC = COLS / 32;
+        constexpr bool MASKED = decltype(masked)::value;
+        const int left = seen - j * kTile;  // this row's keys from this tile's first on
+        auto score = [&](uint32_t w, int c) {
+          float s = __uint_as_float(w);
+          if (!plain) s *= a.scale;
+          if constexpr (MASKED) s = c < left ? s : -INFINITY;
+          return s;
+        };
+        auto largest = [&](const uint32_t* sw, int first, int count, float top) {
+          float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};  // four chains
 #pragma unroll
-        for (int c = 0; c < 4; ++c) ld32(s_at + 32 * c, sw + 32 * c);
-        wait_ld();
-        hold<kTile>(sw);
-        float s[kTile];
+          for (int e = 0; e < count; e += 8)
 #pragma unroll
-        for (int c = 0; c < kTile; ++c) s[c] = __uint_as_float(sw[c]);
-        if (!plain) {
+            for (int x = 0; x < 4; ++x)
+              t4[x] = max3(t4[x], score(sw[e + x], first + e + x), score(sw[e + 4 + x], first + e + 4 + x));
+          return max3(max3(t4[0], t4[1], t4[2]), t4[3], -INFINITY);
+        };
+        constexpr bool EXACT = Reference<T>::kExact;
+        uint32_t sw[EXACT ? NC : 2][32];  // all scores, or a chunk and the next
+        float to = m;
+        if (EXACT || j == 0 || __any_sync(0xffffffffu, live && m == -INFINITY)) {
+          float top = -INFINITY;
+          if constexpr (EXACT) {
 #pragma unroll
-          for (int c = 0; c < kTile; ++c) s[c] *= a.scale;
+            for (int c = 0; c < NC; ++c) ld32(s_at + 32 * c, sw[c]);
+            wait_ld();
+            hold<COLS>(sw[0]);
+            top = largest(sw[0], 0, COLS, top);
+          } else {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              ld32(s_at + 32 * c, sw[0]);
+              wait_ld();
+              hold<32>(sw[0]);
+              top = largest(sw[0], 32 * c, 32, top);
+            }
+          }
+          if (top * k - m > kSlack) to = top * k;  // the first tile too: m is -inf
+        } else if (last > kMost) {
+          to = m + __log2f(last);
         }
-        if (j >= clear) {
-          const int left = seen - j * kTile;  // this row's keys from this tile's first on
-#pragma unroll
-          for (int c = 0; c < kTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
-        }
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c < kTile; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k;
-        const bool moves = mx - m > kSlack;  // the first tile too: m is -inf
-        if (__any_sync(0xffffffffu, moves)) {
-          const float to = moves ? mx : m;
-          const float f = moves ? ex2(m - to) : 1.f;
+        if (__any_sync(0xffffffffu, to != m)) {
+          const float f = to != m ? ex2(m - to) : 1.f;
           m = to;
           l *= f;
           if (j > 0) {  // S of this step is there, so the product of the last one is done
@@ -294,28 +333,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ref = m == -INFINITY ? 0.f : m;
         const float2 k2 = make_float2(k, k), r2 = make_float2(-ref, -ref);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if constexpr (!EXACT) {
+          ld32(s_at, sw[0]);
+          wait_ld();
+          hold<32>(sw[0]);
+        }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < NC; ++c) {
+          if (!EXACT && c + 1 < NC) ld32(s_at + 32 * (c + 1), sw[(c + 1) & 1]);  // on its way meanwhile
+          const uint32_t* now = sw[EXACT ? c : c & 1];
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int x = 32 * c + 2 * e;
-            float2 v = fma2(make_float2(s[x], s[x + 1]), k2, r2);
+            float2 v = fma2(make_float2(score(now[2 * e], x), score(now[2 * e + 1], x + 1)), k2, r2);
             v.x = ex2(v.x);
             v.y = ex2(v.y);
             sum[e & 1] = add2(sum[e & 1], v);
             // the weights round to the values' type, as the tensor core wants them; the sum does not
             pw[e] = Elem<T>::pack(v.x, v.y);
           }
-          st16(s_at + 16 * c, pw);
+          auto announce = [&](uint64_t* bar) {
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+          };
+          // the first 64 keys' weights are announced a chunk late, when their store has long finished
+          if (c == 2) announce(&p_most[i]);
+          st16(s_at + 16 * c, pw);  // over scores that are read
+          if (c + 1 < NC) {
+            if constexpr (!EXACT) {
+              wait_ld();
+              hold<32>(sw[(c + 1) & 1]);
+            }
+          } else {
+            if (NC < 3) announce(&p_most[i]);
+            announce(&p_full[i]);
+          }
         }
-        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
-        wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        last = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        l += last;
+      };
+      for (int j = 0; j < n; ++j, ++steps) {
+        wait_for(&s_full[i], steps & 1, dead);
+        fence_after();
+        if (j < clear)
+          step(j, std::integral_constant<int, kTile>{}, std::false_type{});
+        else if (half_step(it.seen[i], j))
+          step(j, std::integral_constant<int, kTile / 2>{}, std::true_type{});
+        else
+          step(j, std::integral_constant<int, kTile>{}, std::true_type{});
       }
-      if (!ok) break;
       const int h = it.kh * a.rep + rhead;
       uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2);
       if (n == 0) {  // no key for any row of the tile
@@ -325,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         continue;
       }
-      if (!(ok = wait_for(&o_full[i], items++ & 1, dead))) break;
+      wait_for(&o_full[i], items++ & 1, dead);
       fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       float odd = 0.f;  // not zero once an element is infinite or NaN
@@ -362,106 +431,116 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ tensor core
-    constexpr uint32_t kType = sizeof(T) == 2 && __is_same(T, __half) ? 0u : 1u;
-    constexpr uint32_t kCommon = (1u << 4) | (kType << 7) | (kType << 10) | ((kTile >> 4) << 24);
-    constexpr uint32_t kScores = kCommon | ((kTile >> 3) << 17);              // K rows along K: as stored
-    constexpr uint32_t kValues = kCommon | (1u << 16) | ((D >> 3) << 17);     // V rows along N: transposed
-    unsigned loads = 0, steps[2] = {0, 0}, items[2] = {0, 0};
-    bool ok = true;
-    auto stage = [&](unsigned x) { return ring + (x % NS) * L::kTileBytes; };
-    auto landed = [&](unsigned x) { return wait_for(&kv_full[x % NS], (x / NS) & 1, dead); };
-    auto scores = [&](int i, uint32_t kt) {
+    constexpr uint32_t kType = __is_same(T, __half) ? 0u : 1u;
+    constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | ((kTile >> 4) << 24);  // K as stored
+    constexpr uint32_t kValues = kScores | (1u << 16) | ((D >> 3) << 17);  // V transposed: its rows run along N
+    const bool leader = elect_one();
+    const uint32_t tm = uniform(tmem);
+    unsigned loads = 0, steps[2] = {0, 0}, items[2] = {0, 0}, tails = 0;  // `tails`: a bit a stage, v_clean's parity
+    auto landed = [&](unsigned x) { wait_for(&kv_full[x % NS], (x / NS) & 1, dead); };
+    auto scores = [&](int i, unsigned x, bool half) {
+      const uint32_t idesc = kScores | ((half ? kTile / 2 : kTile) >> 3) << 17;
+      const uint64_t qd = operand(smem + i * L::kTileBytes, 16), kd = operand(ring + (x % NS) * L::kTileBytes, 16);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        const uint32_t at = (d >> 2) * L::kBox + (d & 3) * 32;
-        mma_ss(tmem + i * kTile, operand(smem + i * L::kTileBytes + at, 16), operand(kt + at, 16), kScores, d > 0);
+        const uint32_t at = ((d >> 2) * L::kBox + (d & 3) * 32) >> 4;
+        mma_ss(leader, tm + i * kTile, qd + at, kd + at, idesc, d > 0);
       }
-      commit(&s_full[i]);
+      commit(leader, &s_full[i]);
     };
-    while (ok && walk.next<PAGED>(a, p, lane, it)) {
-      const int n = max(it.n[0], it.n[1]);
-      if (n == 0) continue;
-      const unsigned base = loads;
+    while (walk.next<PAGED>(a, p, lane, it)) {
+      const int seen[2] = {uniform(it.seen[0]), uniform(it.seen[1])}, len = uniform(it.len);
+      const int tiles[2] = {tiles_of(seen[0]), tiles_of(seen[1])}, n = max(tiles[0], tiles[1]);
+      const unsigned base = loads;  // K_0, V_0, K_1, V_1, ... of the item
       loads += 2 * n;
-      for (int i = 0; ok && i < 2; ++i)
-        if (it.n[i]) ok = wait_for(&q_full[i], items[i] & 1, dead);
-      if (!ok || !(ok = landed(base))) break;
-      if (elect_one()) {
-        for (int i = 0; i < 2; ++i)
-          if (it.n[i]) {
-            scores(i, stage(base));
-            if (it.n[i] == 1) commit(&q_empty[i]);
-          }
-        commit(&kv_empty[base % NS]);
+      if (n == 0) continue;
+      landed(base);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!tiles[i]) continue;
+        wait_for(&q_full[i], items[i] & 1, dead);
+        scores(i, base, half_step(seen[i], 0));
+        if (tiles[i] == 1) commit(leader, &q_empty[i]);
       }
-      __syncwarp();
-      for (int j = 0; ok && j < n; ++j) {
+      commit(leader, &kv_empty[base % NS]);
+      for (int j = 0; j < n; ++j) {
         const unsigned vx = base + 2 * j + 1, kx = vx + 1;
-        bool v_here = false, k_here = false;
+        landed(vx);
+        if (j + 1 < n) landed(kx);
+        if (len - j * kTile < kTile) {
+          wait_for(&v_clean[vx % NS], tails >> (vx % NS) & 1, dead);
+          tails ^= 1u << (vx % NS);
+        }
+        const uint64_t vd = operand(ring + (vx % NS) * L::kTileBytes, L::kBox);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (j >= it.n[i]) continue;
-          if (!v_here) {
-            if (!(ok = landed(vx))) break;
-            v_here = true;
-            const int rows = it.len - j * kTile;
-            if (rows < kTile) {
-              // what lies behind the last key is not this sequence's: zero, or its weight of zero
-              // would make NaN of a NaN
-              for (int x = rows * 8 + lane; x < kTile * 8; x += 32)
-#pragma unroll
-                for (int hf = 0; hf < L::kHalves; ++hf)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage(vx) + hf * L::kBox + x * 16), "r"(0)
-                               : "memory");
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-            }
-          }
-          if (!(ok = wait_for(&p_full[i], steps[i]++ & 1, dead))) break;
-          if (j == 0 && !(ok = wait_for(&o_free[i], (items[i]++ & 1) ^ 1, dead))) break;
-          const bool more = j + 1 < it.n[i];
-          if (more && !k_here) {
-            if (!(ok = landed(kx))) break;
-            k_here = true;
-          }
+          if (j >= tiles[i]) continue;
+          const uint32_t p_at = tm + i * kTile, o_at = tm + 2 * kTile + i * D;
+          const bool more = j + 1 < tiles[i];
+          if (j == 0) wait_for(&o_free[i], (items[i]++ & 1) ^ 1, dead);
+          wait_for(&p_most[i], steps[i] & 1, dead);
           fence_after();
-          if (elect_one()) {
+          auto values = [&](int x) {  // 16 keys
+            mma_ts(leader, o_at, p_at + 8 * x, vd + x * (2048 >> 4), kValues, j > 0 || x > 0);
+          };
+          const bool half = half_step(seen[i], j);
 #pragma unroll
-            for (int x = 0; x < kTile / 16; ++x)
-              mma_ts(tmem + 2 * kTile + i * D, tmem + i * kTile + 8 * x, operand(stage(vx) + x * 2048, L::kBox), kValues,
-                     j > 0 || x > 0);
-            if (more) {
-              scores(i, stage(kx));
-              if (j + 2 == it.n[i]) commit(&q_empty[i]);
-            } else {
-              commit(&o_full[i]);
-            }
+          for (int x = 0; x < 4; ++x) values(x);
+          wait_for(&p_full[i], steps[i]++ & 1, dead);
+          fence_after();
+          if (!half) {
+#pragma unroll
+            for (int x = 4; x < 8; ++x) values(x);
           }
-          __syncwarp();
+          if (more) {
+            scores(i, kx, half_step(seen[i], j + 1));
+            if (j + 2 == tiles[i]) commit(leader, &q_empty[i]);
+          } else {
+            commit(leader, &o_full[i]);
+          }
         }
-        if (ok && elect_one()) {
-          commit(&kv_empty[vx % NS]);
-          if (j + 1 < n) commit(&kv_empty[kx % NS]);
-        }
-        __syncwarp();
+        commit(leader, &kv_empty[vx % NS]);
+        if (j + 1 < n) commit(leader, &kv_empty[kx % NS]);
       }
     }
-    if (elect_one()) commit(&drained);  // before the TMEM is given back
-    __syncwarp();
+    commit(leader, &drained);  // before the TMEM is given back
     drain(&drained, 0);
+    __syncwarp();
+  } else if (warp == kZeroWarp) {
+    // ------------------------------------------------------------------ behind the last value
+    // What lies there is not this sequence's: zero, or its weight of zero would make NaN of a NaN.
+    // v_tail says that the load of such a tile is under way (kv_full alone would not say which of the
+    // stage's loads it speaks of), v_clean that it is ready; the stage is not loaded again before that.
+    unsigned loads = 0, tails = 0;
+    while (walk.next<PAGED>(a, p, lane, it)) {
+      const int n = tiles_of(max(it.seen[0], it.seen[1])), rows = it.len - (n - 1) * kTile;
+      loads += 2 * n;
+      if (n == 0 || rows >= kTile) continue;
+      const unsigned vx = loads - 1, st = vx % NS;
+      wait_for(&v_tail[st], tails >> st & 1, dead);
+      wait_for(&kv_full[st], (vx / NS) & 1, dead);
+      tails ^= 1u << st;
+      for (int x = rows * 8 + lane; x < kTile * 8; x += 32)
+#pragma unroll
+        for (int hf = 0; hf < L::kHalves; ++hf)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * L::kTileBytes + hf * L::kBox + x * 16),
+                       "r"(0) : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_clean[st]);
+    }
   } else if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ loads
     unsigned loads = 0, items[2] = {0, 0};
-    bool ok = true;
     const int rows_q = a.tok * a.rep;
-    while (ok && walk.next<PAGED>(a, p, lane, it)) {
-      const int n = max(it.n[0], it.n[1]);
+    while (walk.next<PAGED>(a, p, lane, it)) {
+      const int n = tiles_of(max(it.seen[0], it.seen[1]));
       const int* table = PAGED ? p.table + it.b * p.table_row : nullptr;
-      for (int j = 0; ok && j < n; ++j) {
+      for (int j = 0; j < n; ++j) {
         for (int kv = 0; kv < 2; ++kv, ++loads) {
           if (j == 0) {  // Q_0, K, Q_1, V: in the order of their use
-            if (it.n[kv]) {
-              if (!(ok = wait_for(&q_empty[kv], (items[kv]++ & 1) ^ 1, dead))) break;
+            if (it.seen[kv]) {
+              wait_for(&q_empty[kv], (items[kv]++ & 1) ^ 1, dead);
               if (elect_one()) {
                 mbar_expect_tx(&q_full[kv], rows_q * 128 * L::kHalves);
 #pragma unroll
@@ -473,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const unsigned st = loads % NS;
-          if (!(ok = wait_for(&kv_empty[st], ((loads / NS) & 1) ^ 1, dead))) break;
+          wait_for(&kv_empty[st], ((loads / NS) & 1) ^ 1, dead);
           const CUtensorMap* map = kv ? &vmap : &kmap;
           const uint32_t dst = ring + st * L::kTileBytes;
           if (PAGED) {
@@ -496,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tma_3d(dst + hf * L::kBox, map, hf * 64, it.kh, it.k0 + j * kTile, &kv_full[st]);
           }
           __syncwarp();
+          if (kv && it.len - j * kTile < kTile && lane == 0) mbar_arrive(&v_tail[st]);
         }
       }
     }

@@ -57,23 +57,35 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
       : "memory");
 }
 
-// D[128, N] (+)= A[128, 16] . B[N, 16]^T, 16-bit in, fp32 out; A in shared memory or in TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// D[128, N] (+)= A[128, 16] . B[N, 16]^T, 16-bit in, fp32 out; A in shared memory or in TMEM. The whole
+// warp runs these with the same operands and `leader` set in one lane, which issues: a branch around
+// them would keep the operands out of the uniform registers that the instruction takes them from.
+__device__ __forceinline__ void mma_ss(bool leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(bool leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)leader)
       : "memory");
 }
-// Arrives on `bar` once every tcgen05.mma that this thread issued before has completed.
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+// Arrives on `bar` once every tcgen05.mma that the leader issued before has completed.
+__device__ __forceinline__ void commit(bool leader, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+      "r"((uint32_t)leader)
+      : "memory");
+}
+// A value that all lanes of a warp hold alike, as one that the compiler knows to be the same in all.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) {
+  return (T)__shfl_sync(0xffffffffu, v, 0);
 }
 
 // Shared-memory operand with the 128-byte swizzle: 8 rows of 128 bytes an atom, atoms 1024 bytes
@@ -103,6 +115,12 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The largest of three (of those that are no NaN).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
