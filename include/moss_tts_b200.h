@@ -409,16 +409,21 @@ int mt_paged_attention_decode(const void* q, int q_row, int q_head, const mt_pag
  * in elements; sequence b holds query rows cu_q[b] .. cu_q[b + 1] - 1 and key rows cu_k[b] ..
  * cu_k[b + 1] - 1 (int32 [batch + 1]). The last query stands at the last key: with causal != 0, query
  * i of n sees keys 0 .. len - n + i, which for len < n leaves the first rows without a key (zeros).
- * out [tokens_q][nq][D]; rows outside every sequence are left as they were.
+ * out [tokens_q][nq][D]; rows outside every sequence are left as they were. `workspace`:
+ * mt_prompt_attention_workspace bytes (0 where the call's sizes need none; `keys` = tokens_k, or max_pages *
+ * page_size), 16-byte aligned, of any content, one for each call that may run at once; NULL does without, to
+ * the cost of calls with few rows and many keys.
  */
+int mt_prompt_attention_workspace(int tokens, int batch, int keys, int nq, int nkv, int head_dim, long long* bytes);
 int mt_packed_attention(const void* q, int q_row, int q_head, const void* k, int k_row, int k_head, const void* v,
                         int v_row, int v_head, const void* cu_q, const void* cu_k, int batch, int tokens_q,
                         int tokens_k, int nq, int nkv, int head_dim, int type, int causal, float scale, void* out,
-                        int flags, void* stream);
+                        void* workspace, int flags, void* stream);
 
 /* mt_packed_attention, causal, of the newest cu_seqlens[b + 1] - cu_seqlens[b] tokens over pages. */
 int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const mt_paged_kv* kv, const void* cu_seqlens,
-                              int tokens, int nq, float scale, void* out, void* status, int flags, void* stream);
+                              int tokens, int nq, float scale, void* out, void* workspace, void* status, int flags,
+                              void* stream);
 
 /*
  * Output heads of one decode step with greedy selection: final add_rmsnorm of

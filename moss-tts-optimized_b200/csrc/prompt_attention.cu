@@ -13,10 +13,10 @@
 //             for 64, so this thread does nothing else: its every wait shows in the tensor core
 //   9         loads Q, and K and V tiles through a ring, by TMA with the 128-byte swizzle
 //   10        zeroes the rows behind a sequence's last value
-//   11        fills up the third warpgroup, whose registers go to the softmax warps
+//   11        asks for the next item
 // TMEM: S_0 | S_1 | O_0 | O_1; P_i overwrites S_i (16-bit, half its columns) once its row is in
 // registers. While one tile's softmax runs, the tensor core works for the other.
-#include <type_traits>
+#include <type_traits>  // integral_constant
 
 #include "paged.cuh"
 #include "tensor_core.cuh"
@@ -35,22 +35,23 @@ using pipe::mbar_try_wait;
 __device__ int g_prompt_error;  // set when a bounded wait expired (read through mt_read_error_word)
 
 constexpr int kTile = 128;      // query rows of a tile and keys of a step
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10, kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10, kFeedWarp = 11, kThreads = 384;
+constexpr int kWalkers = 11;    // warps that take an item from the feed
 constexpr int kTmemCols = 512;
 // A row that needs the slow path (below) keeps its warp busy for long; far above that all the same.
 constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
-// The reference m that a row's exponentials are taken against is the largest score of its first tile,
-// and then moves only when it has to: weights far above 1 lose nothing in fp32 sums and 16-bit floating
-// weights, and an accumulator is rescaled once or twice a row instead of at every new maximum.
-// With bf16 weights, whose range is that of fp32, it moves when a step's weights add up to more than
-// kMost, for the next step: no maximum is looked for after the first tile. Scores that rise by 2^127
-// within one step leave an infinity, and the row is computed again (row_again). fp16 weights end at
-// 2^16: there the maximum is found in every step before the weights are, and m follows it when it is
-// 2^kSlack above.
-constexpr float kSlack = 8.f, kMost = 256.f;
+// The reference m that a row's exponentials are taken against need not be the largest score: weights far
+// above 1 lose nothing in fp32 sums and 16-bit floating weights. It begins at the row's first score and
+// moves when a step's weights add up to more than `most`, for the next step, which rescales the
+// accumulator (seldom: the largest of many scores is rarely far above the first). No maximum is looked for.
+//   bf16 weights have the range of fp32: scores that rise by 2^97 within one step leave an infinity, and
+//   the row is computed again (row_again).
+//   fp16 weights end at 2^16: a step whose weights add up to more than `fits` is taken again with its
+//   maximum, before the weights go out; they go out all at once.
 template <typename T>
 struct Reference {
-  static constexpr bool kExact = __is_same(T, __half);
+  static constexpr bool kChecked = __is_same(T, __half);
+  static constexpr float most = kChecked ? 256.f : 1073741824.f, fits = 32768.f;
 };
 
 struct PromptArgs {
@@ -63,6 +64,10 @@ struct PromptArgs {
   int tokens_q, tokens_k, batch, nq, nkv, rep, causal;
   int tok;           // tokens of a query tile: 128 / rep
   float scale;       // scale * log2 e
+  // where items may be cut along their keys: the most pieces there may be, and per piece
+  // [256 rows][D] unnormalised outputs, [256] references, [256] sums
+  int units;
+  float* parts;
 };
 
 // Rows [first, first + n) of sequence b in a packed buffer of `tokens` rows; offsets outside the
@@ -72,10 +77,12 @@ __device__ __forceinline__ void span_of(const int* cu, int b, int tokens, int& f
   n = max(min(cu[b + 1], tokens) - first, 0);
 }
 
-struct Item {
+struct __align__(16) Item {
   int b, kh, q0, lq, k0, len;  // sequence, key head, its rows
   int t0;                      // first token of query tile 0
   int seen[2];                 // keys that query tile i's last row sees
+  int j0, j1;                  // key tiles of this piece of the item: [j0, j1), as far as a query tile reads
+  int none;                    // there is no further item
 };
 // Key tiles of a query tile, and the keys that step j of them works on: 128, or 64 where the last
 // tile holds no more.
@@ -86,27 +93,25 @@ __device__ __forceinline__ int keys_seen(const PromptArgs& a, const Item& it, in
   return a.causal ? min(max(it.len - it.lq + t + 1, 0), it.len) : it.len;
 }
 
-// The items of a CTA in order. Flat item w = (query tile pair, key head), pairs in order of the
-// sequences and, inside one, from its end, where a causal row sees most. CTA c takes the c-th item of
-// even rounds of gridDim and the c-th from the end of odd ones: the costs fall along a sequence, and
-// this evens them out. Every warp walks the list by itself.
-struct Walk {
-  long round = 0;
+// Tile pairs of a sequence of lq new tokens.
+__device__ __forceinline__ int pairs_of(const PromptArgs& a, int lq) { return (lq + 2 * a.tok - 1) / (2 * a.tok); }
+
+// Finds flat item w = (query tile pair, key head); pairs in order of the sequences and, inside one,
+// from its end, where a causal row sees most. By a converged warp; rising indices are found without a new
+// start.
+struct Finder {
   int first = 0;    // 32 sequences from here on are scanned next
   long before = 0;  // tile pairs of the sequences before `first`
 
   template <bool PAGED>
-  __device__ bool next(const PromptArgs& a, const Pages& p, int lane, Item& it) {
-    const long g = gridDim.x;
-    const long w = round * g + ((round & 1) ? g - 1 - blockIdx.x : blockIdx.x);
-    ++round;
-    const long pair = w / a.nkv;
-    it.kh = (int)(w - pair * a.nkv);
+  __device__ bool find(const PromptArgs& a, const Pages& p, int lane, int w, Item& it) {
+    const int pair = w / a.nkv;
+    it.kh = w - pair * a.nkv;
+    if (pair < before) first = 0, before = 0;
     for (; first < a.batch; first += 32) {
       int q0 = 0, lq = 0;
       if (first + lane < a.batch) span_of(a.cu_q, first + lane, a.tokens_q, q0, lq);
-      const int count = (lq + 2 * a.tok - 1) / (2 * a.tok);
-      int upto = count;
+      int upto = pairs_of(a, lq);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -129,6 +134,8 @@ struct Walk {
           const int t = it.t0 + i * a.tok;
           it.seen[i] = t < it.lq ? keys_seen(a, it, min(t + a.tok, it.lq) - 1) : 0;
         }
+        it.j0 = 0;
+        it.j1 = tiles_of(max(it.seen[0], it.seen[1]));
         return true;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -136,6 +143,32 @@ struct Walk {
     return false;
   }
 };
+
+// Pieces that every item is cut into along its keys, where there are fewer items than half the CTAs: as
+// many as there are CTAs for, of three key tiles or more (a piece costs its accumulator's way through
+// the workspace and a join, about two tiles). By a converged warp.
+template <bool PAGED>
+__device__ int pieces(const PromptArgs& a, const Pages& p, int lane) {
+  long pairs = 0;
+  int longest = 0;
+  for (int b = lane; b < a.batch; b += 32) {
+    int first, lq, len;
+    span_of(a.cu_q, b, a.tokens_q, first, lq);
+    if (PAGED)
+      len = paged::clamped_len(p, b, nullptr);
+    else
+      span_of(a.cu_k, b, a.tokens_k, first, len);
+    pairs += pairs_of(a, lq);
+    if (lq) longest = max(longest, len);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  const long items = max(pairs * a.nkv, 1L);
+  return (int)max(1L, min(a.units / items, (long)(tiles_of(longest) / 3)));
+}
 
 // Waits for a phase. Where that does not come, the kernel gives up: `dead` ends this and every later
 // wait at once, and the warps run through what is left of their work, to no use but within bounds.
@@ -195,7 +228,7 @@ struct Layout {
   static constexpr uint32_t kBytes = (2 + kStages) * kTileBytes + 1024;
 };
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_tiles(const __grid_constant__ PromptArgs a, const __grid_constant__ Pages p, const __grid_constant__ CUtensorMap qmap,
                  const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -204,6 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_most[2], p_full[2], o_full[2], o_free[2];
   __shared__ __align__(8) uint64_t kv_full[NS], kv_empty[NS], v_tail[NS], v_clean[NS], drained;
+  __shared__ uint4 answer;  // which block's item comes next
+  __shared__ Item item_s;
+  __shared__ __align__(8) uint64_t answered, item_full, item_empty;
   __shared__ uint32_t tmem_s;
   __shared__ int dead_s;
   volatile int* dead = &dead_s;
@@ -231,6 +267,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&v_tail[i], 1);
         mbar_init(&v_clean[i], 1);
       }
+      mbar_init(&answered, 1);
+      mbar_init(&item_full, 1);
+      mbar_init(&item_empty, kWalkers);
       mbar_init(&drained, 1);
       dead_s = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -243,13 +282,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  // 168 registers a thread at launch: 2 x 200 for the softmax warpgroups, 104 for the third
+  // 168 registers a thread at launch, three warpgroups: the softmax's two take from the third
+  constexpr int kSoftmaxRegs = 200, kOtherRegs = 3 * 168 - 2 * kSoftmaxRegs;
   if (warp < kMmaWarp)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
   else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  Walk walk;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   Item it;
+  unsigned taken = 0;  // items of this CTA so far
+  auto next = [&]() -> bool {  // the next item, as the feed warp has laid it out
+    wait_for(&item_full, taken++ & 1, dead);
+    const int4 *from = reinterpret_cast<const int4*>(&item_s);
+    int4 *to = reinterpret_cast<int4*>(&it);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) to[x] = from[x];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty);
+    return !*dead && !it.none;
+  };
   if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ softmax, one thread a row
     const int i = warp >> 2, row = threadIdx.x & 127;
@@ -261,12 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // belongs to the largest score
     const bool plain = a.scale > 0.f;
     const float k = plain ? a.scale : 1.f;
-    while (walk.next<PAGED>(a, p, lane, it)) {
+    while (next()) {
       const int t = it.t0 + i * a.tok + rtok;  // this row's token
       const bool live = rtok < a.tok && t < it.lq;
-      const int n = tiles_of(it.seen[i]), seen = live ? keys_seen(a, it, t) : 0;
+      const int n = min(tiles_of(it.seen[i]), it.j1), seen = live ? keys_seen(a, it, t) : 0;  // key tiles [j0, n)
       // tiles that end before the first row's last key need no mask (rows without a token never count)
-      const int clear = n ? keys_seen(a, it, it.t0 + i * a.tok) / kTile : 0;
+      const int clear = it.seen[i] ? keys_seen(a, it, it.t0 + i * a.tok) / kTile : 0;
       float m = -INFINITY, l = 0.f;
       float last = 0.f;  // the sum of the last step's weights
       // One step: a tile of scores to weights. COLS of its keys, MASKED where a row sees fewer.
@@ -280,102 +330,123 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (MASKED) s = c < left ? s : -INFINITY;
           return s;
         };
-        auto largest = [&](const uint32_t* sw, int first, int count, float top) {
-          float t4[4] = {top, -INFINITY, -INFINITY, -INFINITY};  // four chains
-#pragma unroll
-          for (int e = 0; e < count; e += 8)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              t4[x] = max3(t4[x], score(sw[e + x], first + e + x), score(sw[e + 4 + x], first + e + 4 + x));
-          return max3(max3(t4[0], t4[1], t4[2]), t4[3], -INFINITY);
-        };
-        constexpr bool EXACT = Reference<T>::kExact;
-        uint32_t sw[EXACT ? NC : 2][32];  // all scores, or a chunk and the next
-        float to = m;
-        if (EXACT || j == 0 || __any_sync(0xffffffffu, live && m == -INFINITY)) {
-          float top = -INFINITY;
-          if constexpr (EXACT) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) ld32(s_at + 32 * c, sw[c]);
-            wait_ld();
-            hold<COLS>(sw[0]);
-            top = largest(sw[0], 0, COLS, top);
-          } else {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              ld32(s_at + 32 * c, sw[0]);
-              wait_ld();
-              hold<32>(sw[0]);
-              top = largest(sw[0], 32 * c, 32, top);
-            }
-          }
-          if (top * k - m > kSlack) to = top * k;  // the first tile too: m is -inf
-        } else if (last > kMost) {
-          to = m + __log2f(last);
-        }
-        if (__any_sync(0xffffffffu, to != m)) {
-          const float f = to != m ? ex2(m - to) : 1.f;
-          m = to;
+        constexpr bool CHECKED = Reference<T>::kChecked;
+        auto move = [&](bool moves, float to) {  // of the rows that do, to another reference
+          const float f = moves ? ex2(m - to) : 1.f;
+          if (moves) m = to;
           l *= f;
-          if (j > 0) {  // S of this step is there, so the product of the last one is done
+          if (j == it.j0) return;
+          // S of this step is there, so the product of the last one is done
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t ow[32];
-              ld32(o_at + 32 * c, ow);
-              wait_ld();
-              hold<32>(ow);
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t ow[32];
+            ld32(o_at + 32 * c, ow);
+            wait_ld();
+            hold<32>(ow);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
-              st32(o_at + 32 * c, ow);
-            }
+            for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
+            st32(o_at + 32 * c, ow);
           }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        const float2 k2 = make_float2(k, k), r2 = make_float2(-ref, -ref);
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        if constexpr (!EXACT) {
-          ld32(s_at, sw[0]);
-          wait_ld();
-          hold<32>(sw[0]);
-        }
+        };
+        auto maximum = [&]() {
+          float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (!EXACT && c + 1 < NC) ld32(s_at + 32 * (c + 1), sw[(c + 1) & 1]);  // on its way meanwhile
-          const uint32_t* now = sw[EXACT ? c : c & 1];
-          uint32_t pw[16];
+          for (int c = 0; c < NC; ++c) {
+            uint32_t w[32];
+            ld32(s_at + 32 * c, w);
+            wait_ld();
+            hold<32>(w);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) top = max3(top, score(w[e], 32 * c + e), score(w[e + 1], 32 * c + e + 1));
+          }
+          return top * k;
+        };
+        const float2 k2 = make_float2(k, k);
+        float2 sum[2];
+        uint32_t sw[2][32];  // a chunk of scores and the next
+        auto load = [&](int c) { ld32(s_at + 32 * c, sw[c & 1]); };
+        auto arrived = [&](int c) {
+          wait_ld();
+          hold<32>(sw[c & 1]);
+        };
+        auto weights = [&](int c, float ref, uint32_t* pw) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int x = 32 * c + 2 * e;
-            float2 v = fma2(make_float2(score(now[2 * e], x), score(now[2 * e + 1], x + 1)), k2, r2);
+            float2 v = fma2(make_float2(score(sw[c & 1][2 * e], x), score(sw[c & 1][2 * e + 1], x + 1)), k2,
+                            make_float2(-ref, -ref));
             v.x = ex2(v.x);
             v.y = ex2(v.y);
             sum[e & 1] = add2(sum[e & 1], v);
             // the weights round to the values' type, as the tensor core wants them; the sum does not
             pw[e] = Elem<T>::pack(v.x, v.y);
           }
-          auto announce = [&](uint64_t* bar) {
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-          };
-          // the first 64 keys' weights are announced a chunk late, when their store has long finished
-          if (c == 2) announce(&p_most[i]);
-          st16(s_at + 16 * c, pw);  // over scores that are read
-          if (c + 1 < NC) {
-            if constexpr (!EXACT) {
-              wait_ld();
-              hold<32>(sw[(c + 1) & 1]);
+        };
+        auto announce = [&](uint64_t* bar) {
+          wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        };
+        auto total = [&]() { return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y); };
+
+        if (__any_sync(0xffffffffu, last > Reference<T>::most)) move(last > Reference<T>::most, m + __log2f(last));
+        load(0);
+        arrived(0);
+        if (j == it.j0) {
+          m = score(sw[0][0], 0) * k;
+        } else if (__any_sync(0xffffffffu, live && m == -INFINITY)) {  // no key seen yet, or infinitely low ones
+          const float to = maximum();
+          move(m == -INFINITY && to > m, to);
+          load(0);
+          arrived(0);
+        }
+        sum[0] = sum[1] = make_float2(0.f, 0.f);
+        if constexpr (CHECKED) {
+          uint32_t pw[COLS / 2];
+#pragma unroll 1
+          for (int taken_again = 0;; taken_again = 1) {
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              if (c + 1 < NC) load(c + 1);  // on its way meanwhile
+              weights(c, ref, pw + 16 * c);
+              if (c + 1 < NC) arrived(c + 1);
             }
-          } else {
-            if (NC < 3) announce(&p_most[i]);
-            announce(&p_full[i]);
+            if (taken_again || !__any_sync(0xffffffffu, total() > Reference<T>::fits)) break;
+            const float to = maximum();
+            move(to > m, to);
+            sum[0] = sum[1] = make_float2(0.f, 0.f);
+            load(0);
+            arrived(0);
+          }
+#pragma unroll
+          for (int c = 0; c < NC / 2; ++c) st32(s_at + 32 * c, pw + 32 * c);
+          announce(&p_most[i]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[i]);
+        } else {
+          const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            if (c + 1 < NC) load(c + 1);  // on its way meanwhile
+            uint32_t pw[16];
+            weights(c, ref, pw);
+            // the first 64 keys' weights are announced a chunk late, when their store has long finished
+            if (c == 2) announce(&p_most[i]);
+            st16(s_at + 16 * c, pw);  // over scores that are read
+            if (c + 1 < NC) {
+              arrived(c + 1);
+            } else {
+              if (NC < 3) announce(&p_most[i]);
+              announce(&p_full[i]);
+            }
           }
         }
-        last = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+        last = total();
         l += last;
       };
-      for (int j = 0; j < n; ++j, ++steps) {
+      for (int j = it.j0; j < n; ++j, ++steps) {
         wait_for(&s_full[i], steps & 1, dead);
         fence_after();
         if (j < clear)
@@ -386,11 +457,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           step(j, std::integral_constant<int, kTile>{}, std::true_type{});
       }
       const int h = it.kh * a.rep + rhead;
-      uint4* dst = reinterpret_cast<uint4*>(a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2);
+      if constexpr (SPLIT) {
+        // a piece: the accumulator, the reference and the sum as they are
+        float* part = a.parts + (long long)blockIdx.x * (2 * kTile) * (D + 2);
+        const int r = i * kTile + row;
+        const bool none = n <= it.j0 || l == 0.f;  // nothing to add; -inf says so
+        part[2 * kTile * D + r] = none ? -INFINITY : m == -INFINITY ? 0.f : m;
+        part[2 * kTile * (D + 1) + r] = none ? 0.f : l;
+        if (n <= it.j0) continue;
+        wait_for(&o_full[i], items++ & 1, dead);
+        fence_after();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t ow[32];
+          ld32(o_at + 32 * c, ow);
+          wait_ld();
+          hold<32>(ow);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              store32(part + r * D + 32 * c + 8 * e, reinterpret_cast<const uint32_t(&)[8]>(ow[8 * e]));
+          }
+        }
+        continue;
+      }
+      char* dst = a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2;
       if (n == 0) {  // no key for any row of the tile
         if (live) {
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < D / 16; ++c) store32(dst + 32 * c, {0, 0, 0, 0, 0, 0, 0, 0});
         }
         continue;
       }
@@ -406,15 +501,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         hold<32>(ow);
         if (live) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float f[8];
+          for (int e = 0; e < 2; ++e) {  // 32 bytes a store, the most there is: rows lie apart
+            uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-              f[x] = __uint_as_float(ow[8 * e + x]) * inv;
-              odd = fmaf(f[x], 0.f, odd);
+              const float f0 = __uint_as_float(ow[16 * e + 2 * x]) * inv, f1 = __uint_as_float(ow[16 * e + 2 * x + 1]) * inv;
+              odd = fmaf(f0, 0.f, fmaf(f1, 0.f, odd));
+              w[x] = Elem<T>::pack(f0, f1);
             }
-            dst[4 * c + e] = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]),
-                                        Elem<T>::pack(f[6], f[7]));
+            store32(dst + 64 * c + 32 * e, w);
           }
         }
       }
@@ -448,25 +543,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(leader, &s_full[i]);
     };
-    while (walk.next<PAGED>(a, p, lane, it)) {
+    while (next()) {
       const int seen[2] = {uniform(it.seen[0]), uniform(it.seen[1])}, len = uniform(it.len);
-      const int tiles[2] = {tiles_of(seen[0]), tiles_of(seen[1])}, n = max(tiles[0], tiles[1]);
-      const unsigned base = loads;  // K_0, V_0, K_1, V_1, ... of the item
-      loads += 2 * n;
-      if (n == 0) continue;
+      const int j0 = uniform(it.j0), j1 = uniform(it.j1);
+      const int tiles[2] = {min(tiles_of(seen[0]), j1), min(tiles_of(seen[1]), j1)};  // key tiles [j0, tiles[i])
+      if (j1 <= j0) continue;
+      const unsigned base = loads;  // K, V, K, V, ... of the item
+      loads += 2 * (j1 - j0);
       landed(base);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (!tiles[i]) continue;
+        if (tiles[i] <= j0) continue;
         wait_for(&q_full[i], items[i] & 1, dead);
-        scores(i, base, half_step(seen[i], 0));
-        if (tiles[i] == 1) commit(leader, &q_empty[i]);
+        scores(i, base, half_step(seen[i], j0));
+        if (tiles[i] == j0 + 1) commit(leader, &q_empty[i]);
       }
       commit(leader, &kv_empty[base % NS]);
-      for (int j = 0; j < n; ++j) {
-        const unsigned vx = base + 2 * j + 1, kx = vx + 1;
+      for (int j = j0; j < j1; ++j) {
+        const unsigned vx = base + 2 * (j - j0) + 1, kx = vx + 1;
         landed(vx);
-        if (j + 1 < n) landed(kx);
+        if (j + 1 < j1) landed(kx);
         if (len - j * kTile < kTile) {
           wait_for(&v_clean[vx % NS], tails >> (vx % NS) & 1, dead);
           tails ^= 1u << (vx % NS);
@@ -477,13 +573,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j >= tiles[i]) continue;
           const uint32_t p_at = tm + i * kTile, o_at = tm + 2 * kTile + i * D;
           const bool more = j + 1 < tiles[i];
-          if (j == 0) wait_for(&o_free[i], (items[i]++ & 1) ^ 1, dead);
-          wait_for(&p_most[i], steps[i] & 1, dead);
-          fence_after();
           auto values = [&](int x) {  // 16 keys
-            mma_ts(leader, o_at, p_at + 8 * x, vd + x * (2048 >> 4), kValues, j > 0 || x > 0);
+            mma_ts(leader, o_at, p_at + 8 * x, vd + x * (2048 >> 4), kValues, j > j0 || x > 0);
           };
           const bool half = half_step(seen[i], j);
+          if (j == j0) wait_for(&o_free[i], (items[i]++ & 1) ^ 1, dead);
+          wait_for(&p_most[i], steps[i] & 1, dead);
+          fence_after();
 #pragma unroll
           for (int x = 0; x < 4; ++x) values(x);
           wait_for(&p_full[i], steps[i]++ & 1, dead);
@@ -500,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         commit(leader, &kv_empty[vx % NS]);
-        if (j + 1 < n) commit(leader, &kv_empty[kx % NS]);
+        if (j + 1 < j1) commit(leader, &kv_empty[kx % NS]);
       }
     }
     commit(leader, &drained);  // before the TMEM is given back
@@ -512,10 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // v_tail says that the load of such a tile is under way (kv_full alone would not say which of the
     // stage's loads it speaks of), v_clean that it is ready; the stage is not loaded again before that.
     unsigned loads = 0, tails = 0;
-    while (walk.next<PAGED>(a, p, lane, it)) {
-      const int n = tiles_of(max(it.seen[0], it.seen[1])), rows = it.len - (n - 1) * kTile;
-      loads += 2 * n;
-      if (n == 0 || rows >= kTile) continue;
+    while (next()) {
+      const int rows = it.len - (it.j1 - 1) * kTile;
+      if (it.j1 <= it.j0) continue;
+      loads += 2 * (it.j1 - it.j0);
+      if (rows >= kTile) continue;
       const unsigned vx = loads - 1, st = vx % NS;
       wait_for(&v_tail[st], tails >> st & 1, dead);
       wait_for(&kv_full[st], (vx / NS) & 1, dead);
@@ -533,13 +630,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ loads
     unsigned loads = 0, items[2] = {0, 0};
     const int rows_q = a.tok * a.rep;
-    while (walk.next<PAGED>(a, p, lane, it)) {
-      const int n = tiles_of(max(it.seen[0], it.seen[1]));
+    while (next()) {
       const int* table = PAGED ? p.table + it.b * p.table_row : nullptr;
-      for (int j = 0; j < n; ++j) {
+      for (int j = it.j0; j < it.j1; ++j) {
         for (int kv = 0; kv < 2; ++kv, ++loads) {
-          if (j == 0) {  // Q_0, K, Q_1, V: in the order of their use
-            if (it.seen[kv]) {
+          if (j == it.j0) {  // Q_0, K, Q_1, V: in the order of their use
+            if (tiles_of(it.seen[kv]) > it.j0) {
               wait_for(&q_empty[kv], (items[kv]++ & 1) ^ 1, dead);
               if (elect_one()) {
                 mbar_expect_tx(&q_full[kv], rows_q * 128 * L::kHalves);
@@ -584,6 +680,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i)
         if (items[i]) drain(&q_full[i], (items[i] - 1) & 1);
     }
+  } else {
+    // ------------------------------------------------------------------ feed
+    // The first item is this block's own. Each further one belongs to a block that then never starts:
+    // a CTA that is done early takes more, with no counter in memory. It is asked for when all warps
+    // have begun the last one, not sooner: what is taken early is work that no idle CTA can take.
+    Finder finder;
+    for (unsigned n = 0;; ++n) {
+      int w = blockIdx.x, cut = 1;
+      if constexpr (SPLIT) {
+        cut = pieces<PAGED>(a, p, lane);
+        w = n ? -1 : w / cut;
+      } else if (n) {
+        wait_for(&item_empty, (n - 1) & 1, dead);
+        if (*dead) break;
+        if (lane == 0) {
+          mbar_expect_tx(&answered, 16);
+          take_block(&answer, &answered);
+        }
+        __syncwarp();
+        wait_for(&answered, (n - 1) & 1, dead);
+        w = taken_block(&answer);
+      }
+      it.none = w < 0 || !finder.find<PAGED>(a, p, lane, w, it);
+      if constexpr (SPLIT) {
+        if (n) wait_for(&item_empty, (n - 1) & 1, dead);
+        const int piece = blockIdx.x - w * cut, tiles = it.j1;
+        it.j0 = (int)((long)tiles * piece / cut);
+        it.j1 = (int)((long)tiles * (piece + 1) / cut);
+      }
+      if (lane == 0) {
+        item_s = it;
+        mbar_arrive(&item_full);
+      }
+      if (it.none) break;
+    }
+    if (*dead) drain(&answered, 0), drain(&answered, 1);
   }
   fence_before();
   __syncthreads();
@@ -594,6 +726,58 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Joins the pieces of the items, a warp a row:  m = max m_i,
+// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i, pieces in the order of the keys.
+constexpr int kJoinRows = 8;  // of a block
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(32 * kJoinRows) prompt_join(const __grid_constant__ PromptArgs a, const __grid_constant__ Pages p) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+  const int cut = pieces<PAGED>(a, p, lane), tile = r / kTile, rtok = (r % kTile) / a.rep, rhead = r % kTile - rtok * a.rep;
+  Finder finder;
+  Item it;
+  if (!finder.find<PAGED>(a, p, lane, blockIdx.x, it)) return;  // one block column an item
+  const int t = it.t0 + tile * a.tok + rtok;
+  if (rtok >= a.tok || t >= it.lq) return;
+  const int h = it.kh * a.rep + rhead, seen = keys_seen(a, it, t);
+  const float* part = a.parts + (long long)blockIdx.x * cut * (2 * kTile) * (D + 2);
+  auto at = [&](int i) { return part + (long long)i * (2 * kTile) * (D + 2); };
+  float m = -INFINITY;
+  for (int i = lane; i < cut; i += 32) m = fmaxf(m, at(i)[2 * kTile * D + r]);
+  m = warp_max(m);
+  float l = 0.f, o[E] = {};
+  for (int i = 0; i < cut; ++i) {
+    const float mi = at(i)[2 * kTile * D + r];
+    if (mi == -INFINITY) continue;
+    const float f = ex2(mi - m);
+    l = fmaf(f, at(i)[2 * kTile * (D + 1) + r], l);
+    const float* x = at(i) + r * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(x + e);
+      o[e] = fmaf(f, v.x, o[e]);
+      o[e + 1] = fmaf(f, v.y, o[e + 1]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float odd = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    o[e] *= inv;
+    odd = fmaf(o[e], 0.f, odd);
+  }
+  if (__any_sync(0xffffffffu, !(odd == 0.f))) {
+    row_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, seen, it.q0 + t, h);
+    return;
+  }
+  uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2) + lane * (E / 2);
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e], o[2 * e + 1]);
+}
+
+// The most items that a call can have, whatever its sequences' lengths.
+static long long items_most(const PromptArgs& a) { return ((long long)a.tokens_q / (2 * a.tok) + a.batch) * a.nkv; }
 // Query map: boxes of 64 elements x rep heads x 128 / rep tokens. Keys and values: 64 elements x up to
 // 128 rows of one head, of a page or of the packed rows.
 template <typename T, int D, bool PAGED>
@@ -620,22 +804,35 @@ static cudaError_t launch_tiles(const PromptArgs& a, const Pages& p, cudaStream_
     ok = ok && tensor_map(&km, fp16, 3, a.k, d, ks, box) && tensor_map(&vm, fp16, 3, a.v, d, vs, box);
   }
   if (!ok) return cudaErrorInvalidValue;
-  const long long most = ((long long)a.tokens_q / (2 * a.tok) + a.batch) * a.nkv;  // items at the most
-  const int ctas = (int)(most < sm_count() ? most : sm_count());
-  return launch(prompt_tiles<T, D, PAGED>, dim3(ctas), dim3(kThreads), L::kBytes, s, flags, a, p, qm, km, vm);
+  if (a.parts) {
+    const cudaError_t e = launch(prompt_tiles<T, D, PAGED, true>, dim3(a.units), dim3(kThreads), L::kBytes, s, flags, a, p,
+                                 qm, km, vm);
+    return e != cudaSuccess ? e : launch(prompt_join<T, D, PAGED>, dim3((unsigned)items_most(a), 2 * kTile / kJoinRows),
+                                         dim3(32 * kJoinRows), 0, s, flags | kFlagPdl, a, p);
+  }
+  return launch(prompt_tiles<T, D, PAGED, false>, dim3((unsigned)items_most(a)), dim3(kThreads), L::kBytes, s, flags, a, p,
+                qm, km, vm);
 }
 
 template <bool PAGED>
 static cudaError_t launch_prompt(const PromptArgs& a, const Pages& p, int d, int type, cudaStream_t s, int flags) {
+  if (items_most(a) > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (type == 0)
     return d == 128 ? launch_tiles<__nv_bfloat16, 128, PAGED>(a, p, s, flags)
                     : launch_tiles<__nv_bfloat16, 64, PAGED>(a, p, s, flags);
   return d == 128 ? launch_tiles<__half, 128, PAGED>(a, p, s, flags) : launch_tiles<__half, 64, PAGED>(a, p, s, flags);
 }
 
+// Workspace bytes: pieces may be cut where there can be no more items than half the SMs, and keys
+// enough for two pieces (six tiles).
+static long long workspace_of(const PromptArgs& a, long long keys, int d) {
+  if (2 * items_most(a) > sm_count() || keys <= 5 * kTile) return 0;
+  return (long long)sm_count() * (2 * kTile) * (d + 2) * sizeof(float);
+}
+
 static bool query_ok(const void* q, int q_row, int q_head, const void* cu, int tokens, int nq, int nkv, const void* out) {
   return q && cu && out && tokens >= 1 && nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= 64 && q_row > 0 &&
-         q_head > 0 && q_row % 8 == 0 && q_head % 8 == 0 && aligned(q, 16) && aligned(out, 16) && aligned(cu, 4);
+         q_head > 0 && q_row % 8 == 0 && q_head % 8 == 0 && aligned(q, 16) && aligned(out, 32) && aligned(cu, 4);
 }
 
 }  // namespace prompt
@@ -656,33 +853,47 @@ cudaError_t prompt_error_word(int* value, bool clear) {
 
 using namespace mt;
 
+// Workspace bytes of the two calls below: of `batch` sequences with `tokens` query rows in all and up to
+// `keys` keys each.
+MT_API int mt_prompt_attention_workspace(int tokens, int batch, int keys, int nq, int nkv, int head_dim, long long* bytes) {
+  if (!bytes || tokens < 0 || batch < 1 || keys < 0 || nkv < 1 || nq < 1 || nq % nkv || nq / nkv > 64) return kBadArgument;
+  prompt::PromptArgs a = {};
+  a.tokens_q = tokens, a.batch = batch, a.nkv = nkv, a.tok = prompt::kTile / (nq / nkv);
+  *bytes = prompt::workspace_of(a, keys, head_dim);
+  return 0;
+}
+
 // Attention of packed prompts over packed keys and values (see the header).
 MT_API int mt_packed_attention(const void* q, int q_row, int q_head, const void* k, int k_row, int k_head, const void* v,
                                int v_row, int v_head, const void* cu_q, const void* cu_k, int batch, int tokens_q,
                                int tokens_k, int nq, int nkv, int head_dim, int type, int causal, float scale, void* out,
-                               int flags, void* stream) {
+                               void* workspace, int flags, void* stream) {
   if (!prompt::query_ok(q, q_row, q_head, cu_q, tokens_q, nq, nkv, out) || !k || !v || !cu_k) return kBadArgument;
   if (batch < 1 || tokens_k < 1 || (head_dim != 64 && head_dim != 128) || (type != 0 && type != 1)) return kBadArgument;
   if (k_row < 1 || k_head < 1 || v_row < 1 || v_head < 1 || k_row % 8 || k_head % 8 || v_row % 8 || v_head % 8 ||
-      !aligned(k, 16) || !aligned(v, 16) || !aligned(cu_k, 4))
+      !aligned(k, 16) || !aligned(v, 16) || !aligned(cu_k, 4) || !aligned(workspace, 32))
     return kBadArgument;
   const int rep = nq / nkv;
-  const prompt::PromptArgs a{(const char*)q, (const char*)k, (const char*)v, (char*)out, (const int*)cu_q,
-                             (const int*)cu_k, nullptr, q_row, q_head, k_row, k_head, v_row, v_head,
-                             tokens_q, tokens_k, batch, nq, nkv, rep, causal != 0, prompt::kTile / rep,
-                             scale * paged::kLog2e};
+  prompt::PromptArgs a{(const char*)q, (const char*)k, (const char*)v, (char*)out, (const int*)cu_q,
+                       (const int*)cu_k, nullptr, q_row, q_head, k_row, k_head, v_row, v_head,
+                       tokens_q, tokens_k, batch, nq, nkv, rep, causal != 0, prompt::kTile / rep,
+                       scale * paged::kLog2e, sm_count(), nullptr};
+  if (workspace && prompt::workspace_of(a, tokens_k, head_dim)) a.parts = (float*)workspace;
   return prompt::launch_prompt<false>(a, paged::Pages{}, head_dim, type, (cudaStream_t)stream, flags);
 }
 
 // Causal attention of packed prompts over a paged cache (see the header).
 MT_API int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const mt_paged_kv* kv, const void* cu_seqlens,
-                                     int tokens, int nq, float scale, void* out, void* status, int flags, void* stream) {
+                                     int tokens, int nq, float scale, void* out, void* workspace, void* status, int flags,
+                                     void* stream) {
   paged::Pages p;
-  if (!paged::pages_of(kv, &p) || !prompt::query_ok(q, q_row, q_head, cu_seqlens, tokens, nq, kv->heads, out))
+  if (!paged::pages_of(kv, &p) || !prompt::query_ok(q, q_row, q_head, cu_seqlens, tokens, nq, kv->heads, out) ||
+      !aligned(workspace, 32))
     return kBadArgument;
   const int rep = nq / kv->heads;
-  const prompt::PromptArgs a{(const char*)q, nullptr, nullptr, (char*)out, (const int*)cu_seqlens, nullptr, (int*)status,
-                             q_row, q_head, 0, 0, 0, 0, tokens, 0, kv->batch, nq, kv->heads, rep, 1,
-                             prompt::kTile / rep, scale * paged::kLog2e};
+  prompt::PromptArgs a{(const char*)q, nullptr, nullptr, (char*)out, (const int*)cu_seqlens, nullptr, (int*)status,
+                       q_row, q_head, 0, 0, 0, 0, tokens, 0, kv->batch, nq, kv->heads, rep, 1,
+                       prompt::kTile / rep, scale * paged::kLog2e, sm_count(), nullptr};
+  if (workspace && prompt::workspace_of(a, (long long)kv->max_pages * kv->page_size, kv->head_dim)) a.parts = (float*)workspace;
   return prompt::launch_prompt<true>(a, p, kv->head_dim, kv->type, (cudaStream_t)stream, flags);
 }

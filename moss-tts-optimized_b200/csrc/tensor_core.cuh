@@ -111,6 +111,34 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
+// Asks for the index of a block of this grid that has not started, to run it here in its stead; the
+// 16-byte answer completes on `bar`. Not to be asked again after an answer without a block.
+__device__ __forceinline__ void take_block(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block index of an answer, or -1.
+__device__ __forceinline__ int taken_block(const uint4* answer) {
+  int index;
+  asm volatile(
+      "{\n .reg .b64 lo, hi;\n .reg .b128 h;\n .reg .pred p;\n .reg .b32 y, z, w;\n"
+      " ld.shared.v2.b64 {lo, hi}, [%1];\n mov.b128 h, {lo, hi};\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n mov.b32 %0, -1;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n}"
+      : "=r"(index)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return index;
+}
+
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {  // 32 bytes, aligned
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -7,6 +7,8 @@ go to PyTorch's current CUDA stream, outputs are allocated with ``torch.empty``
 (as the reference does), and there is no CPU fallback: the C library must be
 built and the tensors must live on a CUDA device.
 """
+import contextlib
+
 import torch
 
 from . import native
@@ -165,6 +167,7 @@ def qk_rope_decode(qkv, q_weight, k_weight, cos, sin, cache, layer_idx, position
 
 # ---------------------------------------------------------------------------- paged key-value cache
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_HERE = contextlib.nullcontext()
 
 
 def _heads3(name, t, dtype, dev):
@@ -217,8 +220,8 @@ def _out(out, shape, like):
     if out is None:
         return torch.empty(shape, device=like.device, dtype=like.dtype)
     if out.shape != shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() \
-            or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous {like.dtype} tensor {tuple(shape)} on the queries' device")
+            or out.data_ptr() % 32:
+        raise ValueError(f"out must be a contiguous, 32-byte aligned {like.dtype} tensor {tuple(shape)} on the queries' device")
     return out
 
 
@@ -257,22 +260,21 @@ def _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev):
 
 def _call_on(dev, name, *args):
     """``native.call`` on the tensors' device and its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        native.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            native.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    native.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
-def _workspace(size, dev):
-    """A workspace of ``size(device)`` bytes from torch's allocator, for one call: calls on other streams
-    and captured graphs have one each."""
-    if torch.cuda.current_device() == dev.index:
-        n = size(dev.index)
-    else:
-        with torch.cuda.device(dev):
-            n = size(dev.index)
-    return torch.empty(n, device=dev, dtype=torch.uint8)
+def _on(dev):
+    """A context on ``dev`` where that is not the current device."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _workspace(n, dev):
+    """The address of a workspace of ``n`` bytes and the tensor that holds it, from torch's allocator and for
+    one call: calls on other streams and captured graphs have one each."""
+    if not n:
+        return None, None
+    ws = torch.empty(n, device=dev, dtype=torch.uint8)
+    return ws.data_ptr(), ws
 
 
 def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, kv_lens, cu_seqlens, eps, *,
@@ -320,9 +322,10 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     st = _status(status, dev)
     out = _out(out, (tokens, nq, d), qkv)
     if tokens:
-        _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-                 sin.data_ptr(), cos.shape[0], 1 if cos.dtype == torch.float32 else 0, kv, cu, tokens, nq,
-                 max(qkv.stride(0), width), out.data_ptr(), eps, st, 0)
+        with _on(dev):
+            _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
+                     sin.data_ptr(), cos.shape[0], 1 if cos.dtype == torch.float32 else 0, kv, cu, tokens, nq,
+                     max(qkv.stride(0), width), out.data_ptr(), eps, st, 0)
     return out
 
 
@@ -343,9 +346,10 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
         raise ValueError("page_table must have a row for each query row")
     st = _status(status, dev)
     out = _out(out, (batch, nq, d), q)
-    ws = _workspace(native.paged_decode_workspace, dev)
-    _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
-             out.data_ptr(), ws.data_ptr(), st, 0)
+    with _on(dev):
+        at, _ = _workspace(native.paged_decode_workspace(dev.index), dev)
+        _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
+                 out.data_ptr(), at, st, 0)
     return out
 
 
@@ -375,10 +379,14 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, s
         return out
     if k.shape[0] == 0:  # no key anywhere: every row of a sequence is zero, as the kernel would leave it
         k, v, k_row, k_head, v_row, v_head = q, q, row, head, row, head
-        cu_k = torch.zeros(batch + 1, device=dev, dtype=torch.int32).data_ptr()
-    _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
-             v_head, cu_q, cu_k, batch, tokens, max(1, k.shape[0]), nq, k.shape[1], d, _TYPES[q.dtype],
-             1 if causal else 0, d ** -0.5 if scale is None else scale, out.data_ptr(), 0)
+        none = torch.zeros(batch + 1, device=dev, dtype=torch.int32)
+        cu_k = none.data_ptr()
+    tokens_k, nkv = k.shape[0], k.shape[1]
+    with _on(dev):
+        at, _ = _workspace(native.prompt_workspace(tokens, batch, tokens_k, nq, nkv, d), dev)
+        _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+                 v_head, cu_q, cu_k, batch, tokens, tokens_k, nq, nkv, d, _TYPES[q.dtype], 1 if causal else 0,
+                 d ** -0.5 if scale is None else scale, out.data_ptr(), at, 0)
     return out
 
 
@@ -398,6 +406,9 @@ def paged_attention_prompt(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens,
     st = _status(status, dev)
     out = _out(out, (tokens, nq, d), q)
     if tokens:
-        _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
-                 d ** -0.5 if scale is None else scale, out.data_ptr(), st, 0)
+        with _on(dev):
+            most = page_table.shape[1] * k_pages.shape[2]
+            at, _ = _workspace(native.prompt_workspace(tokens, page_table.shape[0], most, nq, k_pages.shape[1], d), dev)
+            _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
+                     d ** -0.5 if scale is None else scale, out.data_ptr(), at, st, 0)
     return out

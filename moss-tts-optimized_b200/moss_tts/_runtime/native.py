@@ -56,8 +56,9 @@ SIGNATURES = {
     "mt_qk_rope_paged": ([_P] * 5 + [_I, _I, _P, _P, _I, _I, _I, _P, _F, _P, _I, _P], _I),
     "mt_paged_attention_decode_workspace": ([_LLP], _I),
     "mt_paged_attention_decode": ([_P, _I, _I, _P, _I, _F, _P, _P, _P, _I, _P], _I),
-    "mt_packed_attention": ([_P, _I, _I] * 3 + [_P, _P] + [_I] * 8 + [_F, _P, _I, _P], _I),
-    "mt_paged_attention_prompt": ([_P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _I, _P], _I),
+    "mt_prompt_attention_workspace": ([_I] * 6 + [_LLP], _I),
+    "mt_packed_attention": ([_P, _I, _I] * 3 + [_P, _P] + [_I] * 8 + [_F, _P, _P, _I, _P], _I),
+    "mt_paged_attention_prompt": ([_P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _P, _I, _P], _I),
     "mt_heads_greedy": ([_P, _P, _P, _F] + [_P] * 11 + [_I] * 11 + [_P], _I),
 }
 
@@ -143,6 +144,13 @@ def paged_decode_workspace(device: int) -> int:
     """Workspace bytes of mt_paged_attention_decode on device ``device`` (the current one)."""
     b = ctypes.c_longlong(0)
     call("mt_paged_attention_decode_workspace", ctypes.byref(b))
+    return b.value
+
+
+def prompt_workspace(tokens: int, batch: int, keys: int, nq: int, nkv: int, head_dim: int) -> int:
+    """Workspace bytes of the packed and paged prompt attention on the current device."""
+    b = ctypes.c_longlong(0)
+    call("mt_prompt_attention_workspace", tokens, batch, keys, nq, nkv, head_dim, ctypes.byref(b))
     return b.value
 
 

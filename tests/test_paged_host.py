@@ -94,7 +94,7 @@ def test_entry_points_refuse_before_a_launch():
                                 dict(size=512), dict(d=96), dict(most=0), dict(batch=0), dict(type=2), dict(lens=P + 2))]
     for x in bad_kv:
         assert lib.mt_paged_attention_decode(P, 256, 64, x, 4, 0.1, P, P, None, 0, None) == 1
-        assert lib.mt_paged_attention_prompt(P, 256, 64, x, P, 2, 4, 0.1, P, None, 0, None) == 1
+        assert lib.mt_paged_attention_prompt(P, 256, 64, x, P, 2, 4, 0.1, P, None, None, 0, None) == 1
         assert lib.mt_qk_rope_paged(P, P, P, P, P, 64, 0, x, P, 2, 4, 512, P, 1e-6, None, 0, None) == 1
     good = kv()
     for a in ((None, 256, 64, good, 4, 0.1, P), (P, 256, 64, good, 3, 0.1, P), (P, 256, 64, good, 0, 0.1, P),
@@ -104,7 +104,7 @@ def test_entry_points_refuse_before_a_launch():
     assert lib.mt_paged_attention_decode(P, 256, 64, good, 4, 0.1, P, None, None, 0, None) == 1  # no workspace
     for a in ((P, 256, 64, P, 128, 64, P, 128, 64, P, P, 0), (P, 256, 64, P, 128, 60, P, 128, 64, P, P, 1),
               (P, 256, 64, P, 128, 64, P, 0, 64, P, P, 1), (P, 256, 64, P, 128, 64, P, 128, 64, None, P, 1)):
-        assert lib.mt_packed_attention(*a, 4, 4, 4, 2, 64, 0, 1, 0.1, P, 0, None) == 1
+        assert lib.mt_packed_attention(*a, 4, 4, 4, 2, 64, 0, 1, 0.1, P, None, 0, None) == 1
     for c in (dict(tokens=0), dict(cu=None, tokens=3), dict(row=504), dict(rows=0), dict(qkv=P + 2), dict(nq=0)):
         f = dict(qkv=P, rows=64, cu=P, tokens=2, nq=4, row=512) | c
         assert lib.mt_qk_rope_paged(f["qkv"], P, P, P, P, f["rows"], 0, good, f["cu"], f["tokens"], f["nq"], f["row"], P,
