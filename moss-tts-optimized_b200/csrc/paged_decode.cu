@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp][head][D]
   long* slab = reinterpret_cast<long*>(merge);  // chunks (of one head) of the sequences before thread t's slab
 
+  if (warp == kConsumers && lane < 2) prefetch_map(lane ? &vmap : &kmap);
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);

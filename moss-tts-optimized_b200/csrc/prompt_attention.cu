@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;  // Q_0, Q_1, then the ring
   const uint32_t ring = smem + 2 * L::kTileBytes;
 
+  if (warp == kLoadWarp && lane < 3) prefetch_map(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
                  "r"(kTmemCols) : "memory");

@@ -7,8 +7,6 @@ go to PyTorch's current CUDA stream, outputs are allocated with ``torch.empty``
 (as the reference does), and there is no CPU fallback: the C library must be
 built and the tensors must live on a CUDA device.
 """
-import contextlib
-
 import torch
 
 from . import native
@@ -166,44 +164,48 @@ def qk_rope_decode(qkv, q_weight, k_weight, cos, sin, cache, layer_idx, position
 
 
 # ---------------------------------------------------------------------------- paged key-value cache
+# A call of a few rows runs for 5 to 10 microseconds on the GPU, and Python's checks are what it waits for:
+# they read every attribute once and compare devices by index.
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
-_HERE = contextlib.nullcontext()
+_DIMS = (64, 128)
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the address alone, without a Stream object
 
 
-def _heads3(name, t, dtype, dev):
+def _strides3(name, t, heads, d):
     """Row and head stride of ``t`` ``[rows, heads, D]``, whose D elements are adjacent."""
-    if t.ndim != 3 or t.dtype != dtype or t.device != dev:
-        raise ValueError(f"{name} must be [rows, heads, D], of the queries' type and device")
-    rows, heads, d = t.shape
     row, head, one = t.stride()
-    if rows <= 1:  # the stride of a dimension of one says nothing
+    if t.shape[0] <= 1:  # the stride of a dimension of one says nothing
         row = heads * d
     if heads <= 1:
         head = d
-    if one != 1 or row % 8 or head % 8 or not 0 < row < 1 << 31 or not 0 < head < 1 << 31 or t.data_ptr() % 16:
+    if one != 1 or (row | head) & 7 or row <= 0 or head <= 0 or row >= 1 << 31 or head >= 1 << 31 or t.data_ptr() & 15:
         raise ValueError(f"{name}: D must be adjacent, rows and heads 16-byte aligned and not broadcast")
     return row, head
 
 
-def _query(q, heads, d):
+def _query(q, nkv, d):
+    """(tokens, heads, row stride, head stride, device index) of the queries."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("CUDA tensors required (there is no CPU path)")
     if q.dtype not in _TYPES:
         raise ValueError("bf16 or fp16 tensors required")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("This attention has no backward pass")
-    row, head = _heads3("q", q, q.dtype, q.device)
-    nq = q.shape[1]
-    if q.shape[2] != d or d not in (64, 128):
+    if q.ndim != 3:
+        raise ValueError("q must be [rows, heads, D]")
+    tokens, nq, dq = q.shape
+    if dq != d or d not in _DIMS:
         raise ValueError("head_dim must be 64 or 128, the same for queries and keys")
-    if nq == 0 or heads == 0 or nq % heads or nq // heads > 64:
+    if nq == 0 or nkv == 0 or nq % nkv or nq // nkv > 64:
         raise ValueError("Query heads must be 1 to 64 times the key heads")
-    return row, head
+    return tokens, nq, *_strides3("q", q, nq, d), q.get_device()
 
 
 def _ints(name, t, n, dev):
-    """An int32 vector of ``n`` elements (lengths or offsets)."""
-    if t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] != n or t.device != dev or not t.is_contiguous():
+    """The address of an int32 vector of ``n`` elements (lengths or offsets)."""
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector of {n} elements on the queries' device")
     return t.data_ptr()
 
@@ -211,7 +213,7 @@ def _ints(name, t, n, dev):
 def _status(status, dev):
     if status is None:
         return None
-    if status.dtype != torch.int32 or status.numel() != 1 or status.device != dev:
+    if status.dtype is not torch.int32 or status.numel() != 1 or status.get_device() != dev:
         raise ValueError("status must be a one-element int32 tensor on the queries' device")
     return status.data_ptr()
 
@@ -219,62 +221,62 @@ def _status(status, dev):
 def _out(out, shape, like):
     if out is None:
         return torch.empty(shape, device=like.device, dtype=like.dtype)
-    if out.shape != shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() \
-            or out.data_ptr() % 32:
-        raise ValueError(f"out must be a contiguous, 32-byte aligned {like.dtype} tensor {tuple(shape)} on the queries' device")
+    if out.shape != shape or out.dtype is not like.dtype or out.get_device() != like.get_device() \
+            or not out.is_contiguous() or out.data_ptr() & 31:
+        raise ValueError(f"out must be a contiguous, 32-byte aligned {like.dtype} tensor {tuple(shape)} on the "
+                         "queries' device")
     return out
 
 
 def _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev):
-    """``mt_paged_kv`` of one layer's pages, as bytes."""
-    if k_pages.ndim != 4 or v_pages.shape != k_pages.shape:
+    """(``mt_paged_kv`` of one layer's pages as bytes, batch, most tokens of a sequence)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must be [pages, heads, page_size, D]")
-    pages, heads, size, d = k_pages.shape
-    if size not in (16, 32, 64, 128, 256):
+    pages, heads, size, d = shape
+    if size not in _PAGE_SIZES:
         raise ValueError("page_size must be a power of two, 16 to 256")
-    if d not in (64, 128):
+    if d not in _DIMS:
         raise ValueError("head_dim must be 64 or 128, the same for queries and keys")
     if pages < 1 or pages >= 1 << 31 or heads < 1:
         raise ValueError("The cache has no pages")
-    strides = []
-    for t in (k_pages, v_pages):
-        if t.dtype != dtype or t.device != dev:
-            raise ValueError("The pages must have the queries' type and device")
-        page, head, row, one = t.stride()
-        if pages == 1:  # the stride of a dimension of one says nothing
-            page = heads * size * d
-        if heads == 1:
-            head = size * d
-        if one != 1 or page % 8 or head % 8 or row % 8 or min(page, head, row) <= 0 or t.data_ptr() % 16:
-            raise ValueError("pages: D must be adjacent, pages, heads and rows 16-byte aligned and not broadcast")
-        strides += (page, head, row)
-    if page_table.dtype != torch.int32 or page_table.ndim != 2 or page_table.device != dev:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype or k_pages.get_device() != dev \
+            or v_pages.get_device() != dev:
+        raise ValueError("The pages must have the queries' type and device")
+    kp, kh, kr, k1 = k_pages.stride()
+    vp, vh, vr, v1 = v_pages.stride()
+    if pages == 1:  # the stride of a dimension of one says nothing
+        kp = vp = heads * size * d
+    if heads == 1:
+        kh = vh = size * d
+    k, v = k_pages.data_ptr(), v_pages.data_ptr()
+    if k1 != 1 or v1 != 1 or (kp | kh | kr | vp | vh | vr) & 7 or (k | v) & 15 or min(kp, kh, kr, vp, vh, vr) <= 0:
+        raise ValueError("pages: D must be adjacent, pages, heads and rows 16-byte aligned and not broadcast")
+    if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.get_device() != dev:
         raise ValueError("page_table must be int32 [batch, max_pages] on the queries' device")
     batch, most = page_table.shape
-    if batch < 1 or most < 1 or most * size > 1 << 30 or page_table.stride(1) != 1:
+    row, one = page_table.stride()
+    if batch < 1 or most < 1 or most * size > 1 << 30 or (one != 1 and most > 1):
         raise ValueError("page_table must have rows of 1 or more adjacent entries, for up to 2^30 tokens")
-    return native.PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-                                _ints("kv_lens", kv_lens, batch, dev), *strides, page_table.stride(0),
-                                pages, heads, size, d, most, batch, _TYPES[dtype])
+    return native.PAGED_KV.pack(k, v, page_table.data_ptr(), _ints("kv_lens", kv_lens, batch, dev), kp, kh, kr, vp, vh,
+                                vr, row, pages, heads, size, d, most, batch, _TYPES[dtype]), batch, most * size
 
 
-def _call_on(dev, name, *args):
-    """``native.call`` on the tensors' device and its current stream."""
-    native.call(name, *args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _call_on(dev, name, *args, workspace=None):
+    """``native.call`` on device ``dev`` and its current stream; ``workspace`` (function, arguments) gives the
+    bytes of a workspace, which comes last before the status, flags and stream. It is taken from torch's
+    allocator for the one call, so that calls on other streams and captured graphs have one each."""
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return _call_on(dev, name, *args, workspace=workspace)
+    if workspace is not None:
+        n = workspace[0](*workspace[1:])
+        held = torch.empty(n, device=torch.device("cuda", dev), dtype=torch.uint8) if n else None
+        args = [held.data_ptr() if a is _WORKSPACE and n else None if a is _WORKSPACE else a for a in args]
+    native.call(name, *args, _raw_stream(dev))
 
 
-def _on(dev):
-    """A context on ``dev`` where that is not the current device."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-def _workspace(n, dev):
-    """The address of a workspace of ``n`` bytes and the tensor that holds it, from torch's allocator and for
-    one call: calls on other streams and captured graphs have one each."""
-    if not n:
-        return None, None
-    ws = torch.empty(n, device=dev, dtype=torch.uint8)
-    return ws.data_ptr(), ws
+_WORKSPACE = object()  # stands for the workspace's address in _call_on's arguments
 
 
 def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, kv_lens, cu_seqlens, eps, *,
@@ -295,37 +297,41 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     """
     if not isinstance(qkv, torch.Tensor) or not qkv.is_cuda:
         raise ValueError("CUDA tensors required (there is no CPU path)")
-    dev, dtype = qkv.device, qkv.dtype
-    if dtype not in _TYPES or qkv.ndim != 2 or qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.stride(0) >= 1 << 31 \
-            or qkv.data_ptr() % 16:
-        raise ValueError("qkv must be bf16 or fp16 [tokens, (nq + 2 nkv) * D] with 16-byte aligned rows")
-    if torch.is_grad_enabled() and qkv.requires_grad:
+    dtype, dev = qkv.dtype, qkv.get_device()
+    if dtype not in _TYPES or qkv.ndim != 2:
+        raise ValueError("qkv must be bf16 or fp16 [tokens, (nq + 2 nkv) * D]")
+    if qkv.requires_grad and torch.is_grad_enabled():
         raise ValueError("This operator has no backward pass")
-    kv = _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev)
     tokens, width = qkv.shape
+    row, one = qkv.stride()
+    if tokens <= 1:
+        row = width
+    if one != 1 or row & 7 or row < width or row >= 1 << 31 or qkv.data_ptr() & 15:
+        raise ValueError("qkv must have adjacent elements in 16-byte aligned rows")
+    kv, batch, _ = _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev)
     nkv, d = k_pages.shape[1], k_pages.shape[3]
     nq = width // d - 2 * nkv
-    if width % d or nq < 1 or (tokens > 1 and qkv.stride(0) < width):
+    if width % d or nq < 1:
         raise ValueError("qkv must hold nq >= 1 query heads and the cache's key and value heads")
     for w in (q_weight, k_weight):
-        if w.shape != (d,) or w.dtype != dtype or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
+        if w.dtype is not dtype or w.shape != (d,) or w.get_device() != dev or not w.is_contiguous() or w.data_ptr() & 15:
             raise ValueError("q_weight and k_weight must be contiguous [D], of qkv's type and device")
-    if cos.ndim != 2 or cos.shape[1] != d or cos.shape[0] < 1 or sin.shape != cos.shape or sin.dtype != cos.dtype:
+    table, kind = cos.shape, cos.dtype
+    if len(table) != 2 or table[1] != d or table[0] < 1 or sin.shape != table:
         raise ValueError("RoPE tables must be [max_len, D]")
-    for t in (cos, sin):
-        if t.dtype not in (dtype, torch.float32) or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError("RoPE tables must be contiguous, in qkv's type or fp32, on its device")
-    batch = page_table.shape[0]
+    if (kind is not dtype and kind is not torch.float32) or sin.dtype is not kind or cos.get_device() != dev \
+            or sin.get_device() != dev or not cos.is_contiguous() or not sin.is_contiguous() \
+            or (cos.data_ptr() | sin.data_ptr()) & 15:
+        raise ValueError("RoPE tables must be contiguous, in qkv's type or fp32, on its device")
     if cu_seqlens is None and tokens != batch:
         raise ValueError("Without cu_seqlens there is one token per sequence")
     cu = None if cu_seqlens is None else _ints("cu_seqlens", cu_seqlens, batch + 1, dev)
     st = _status(status, dev)
     out = _out(out, (tokens, nq, d), qkv)
     if tokens:
-        with _on(dev):
-            _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
-                     sin.data_ptr(), cos.shape[0], 1 if cos.dtype == torch.float32 else 0, kv, cu, tokens, nq,
-                     max(qkv.stride(0), width), out.data_ptr(), eps, st, 0)
+        _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
+                 sin.data_ptr(), table[0], 1 if kind is torch.float32 else 0, kv, cu, tokens, nq, row, out.data_ptr(),
+                 eps, st, 0)
     return out
 
 
@@ -338,18 +344,15 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
     ``status`` as in ``qk_rope_paged``: a length beyond the page table (1) is cut, a page id outside the
     cache (3) reads as zeros.
     """
-    row, head = _query(q, k_pages.shape[1], k_pages.shape[-1])
-    dev = q.device
-    kv = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
-    batch, nq, d = q.shape
-    if page_table.shape[0] != batch:
+    _, nkv, _, d = k_pages.shape
+    rows, nq, row, head, dev = _query(q, nkv, d)
+    kv, batch, _ = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
+    if rows != batch:
         raise ValueError("page_table must have a row for each query row")
     st = _status(status, dev)
     out = _out(out, (batch, nq, d), q)
-    with _on(dev):
-        at, _ = _workspace(native.paged_decode_workspace(dev.index), dev)
-        _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
-                 out.data_ptr(), at, st, 0)
+    _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
+             out.data_ptr(), _WORKSPACE, st, 0, workspace=(native.paged_decode_workspace, dev))
     return out
 
 
@@ -362,14 +365,17 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, s
     at its last key: with ``causal``, query i of n sees keys ``0 .. len - n + i``; a query without a key gives
     zeros. Returns ``[tokens, nq, D]`` (in ``out`` if given); rows outside every sequence are not written.
     """
-    if k.ndim != 3 or v.shape != k.shape:
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape:
         raise ValueError("k and v must be [tokens, nkv, D]")
-    row, head = _query(q, k.shape[1], k.shape[2])
-    dev = q.device
-    k_row, k_head = _heads3("k", k, q.dtype, dev)
-    v_row, v_head = _heads3("v", v, q.dtype, dev)
-    tokens, nq, d = q.shape
-    batch = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.ndim == 1 else 0
+    tokens_k, nkv, d = shape
+    tokens, nq, row, head, dev = _query(q, nkv, d)
+    dtype = q.dtype
+    if k.dtype is not dtype or v.dtype is not dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("k and v must have the queries' type and device")
+    k_row, k_head = _strides3("k", k, nkv, d)
+    v_row, v_head = _strides3("v", v, nkv, d)
+    batch = cu_seqlens_q.numel() - 1
     if batch < 1:
         raise ValueError("cu_seqlens_q must hold batch + 1 offsets of 1 or more sequences")
     cu_q = _ints("cu_seqlens_q", cu_seqlens_q, batch + 1, dev)
@@ -377,16 +383,14 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, s
     out = _out(out, (tokens, nq, d), q)
     if tokens == 0:
         return out
-    if k.shape[0] == 0:  # no key anywhere: every row of a sequence is zero, as the kernel would leave it
-        k, v, k_row, k_head, v_row, v_head = q, q, row, head, row, head
-        none = torch.zeros(batch + 1, device=dev, dtype=torch.int32)
+    if tokens_k == 0:  # no key anywhere: every row of a sequence is zero, as the kernel would leave it
+        k, v, tokens_k, nkv, k_row, k_head, v_row, v_head = q, q, tokens, nq, row, head, row, head
+        none = torch.zeros(batch + 1, device=q.device, dtype=torch.int32)
         cu_k = none.data_ptr()
-    tokens_k, nkv = k.shape[0], k.shape[1]
-    with _on(dev):
-        at, _ = _workspace(native.prompt_workspace(tokens, batch, tokens_k, nq, nkv, d), dev)
-        _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
-                 v_head, cu_q, cu_k, batch, tokens, tokens_k, nq, nkv, d, _TYPES[q.dtype], 1 if causal else 0,
-                 d ** -0.5 if scale is None else scale, out.data_ptr(), at, 0)
+    _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+             v_head, cu_q, cu_k, batch, tokens, tokens_k, nq, nkv, d, _TYPES[dtype], 1 if causal else 0,
+             d ** -0.5 if scale is None else scale, out.data_ptr(), _WORKSPACE, 0,
+             workspace=(native.prompt_workspace, tokens, batch, tokens_k, nq, nkv, d))
     return out
 
 
@@ -398,17 +402,14 @@ def paged_attention_prompt(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens,
     are in the pages already (``qk_rope_paged``). Query i of n sees keys ``0 .. kv_lens[b] - n + i``. Otherwise
     as ``packed_attention``, with ``paged_attention_decode``'s cache and ``status``.
     """
-    row, head = _query(q, k_pages.shape[1], k_pages.shape[-1])
-    dev = q.device
-    kv = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
-    tokens, nq, d = q.shape
-    cu = _ints("cu_seqlens", cu_seqlens, page_table.shape[0] + 1, dev)
+    _, nkv, _, d = k_pages.shape
+    tokens, nq, row, head, dev = _query(q, nkv, d)
+    kv, batch, most = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
+    cu = _ints("cu_seqlens", cu_seqlens, batch + 1, dev)
     st = _status(status, dev)
     out = _out(out, (tokens, nq, d), q)
     if tokens:
-        with _on(dev):
-            most = page_table.shape[1] * k_pages.shape[2]
-            at, _ = _workspace(native.prompt_workspace(tokens, page_table.shape[0], most, nq, k_pages.shape[1], d), dev)
-            _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
-                     d ** -0.5 if scale is None else scale, out.data_ptr(), at, st, 0)
+        _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
+                 d ** -0.5 if scale is None else scale, out.data_ptr(), _WORKSPACE, st, 0,
+                 workspace=(native.prompt_workspace, tokens, batch, most, nq, nkv, d))
     return out

@@ -59,9 +59,9 @@ def _kv(**changes):
     {"kv_lens": ints([20, 0, 30, 0])[::2]},
 ])
 def test_pages_are_checked(change):
-    K._paged(**_kv(), dtype=torch.bfloat16, dev=CPU)
+    K._paged(**_kv(), dtype=torch.bfloat16, dev=-1)
     with pytest.raises(ValueError):
-        K._paged(**_kv(**change), dtype=torch.bfloat16, dev=CPU)
+        K._paged(**_kv(**change), dtype=torch.bfloat16, dev=-1)  # -1: host tensors
 
 
 def test_operators_refuse_host_tensors():
