@@ -4,9 +4,9 @@
 //
 // Bound by HBM: every key and value row is read once, 4 D bytes for 4 D flops a query head. The work is
 // cut into chunks of 64 keys of one key head (and up to 8 of its query heads), laid out one after the
-// other over the sequences, and every CTA takes an equal run of chunks, wherever sequences begin and
-// end: a batch of ragged sequences and one long sequence both load all SMs alike. A run that covers
-// a sequence's head only in part leaves (m, l, o) in the workspace; a second kernel joins the parts,
+// other over the sequences, and every CTA takes a run of chunks, wherever sequences begin and end: a
+// batch of ragged sequences and one long sequence both load all SMs alike. A run that covers a
+// sequence's head only in part leaves (m, l, o) in the workspace; a second kernel joins the parts,
 //   m = max m_i,  o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i,
 // in the order of the keys, so the same inputs give the same bits.
 #include "paged.cuh"
@@ -26,18 +26,56 @@ __device__ int g_paged_error;  // set when a bounded wait expired (read through 
 constexpr int kChunk = 64;      // keys of a chunk
 constexpr int kHeads = 8;       // query heads of an item: rows 0-7 of the mma's 16 (8-15 take the
                                 // low halves of the weights)
-constexpr int kConsumers = 8;   // warps; groups of four take alternate chunks, 16 keys a warp
+constexpr int kConsumers = 4;   // warps, 16 keys of a chunk each
 constexpr int kDecodeThreads = (kConsumers + 1) * 32;
+constexpr int kCtasPerSm = 2;   // one streams while the other begins or ends a run
+// SMs do not get equal shares of HBM: with runs of one length the slowest of 148 ended 16% after the
+// median. Large calls therefore have kRounds runs for every resident CTA, of falling length (shares of 64
+// of the work), which the hardware hands out as CTAs end.
+constexpr int kRounds = 6;
+__constant__ int kShares[kRounds + 1] = {0, 28, 44, 53, 58, 61, 64};
+
+// How `work` chunks are laid out in runs: `rounds` x `width`, none empty.
+struct Plan {
+  long work;
+  int width, rounds;
+  __device__ __forceinline__ Plan(long work, int runs, int rounds_most) : work(work) {
+    width = runs / rounds_most;
+    // the shortest round has 3/64 of the work
+    rounds = rounds_most > 1 && work * 3 >= 64L * (width + 1) ? rounds_most : 1;
+    if (work < width) width = (int)work;
+  }
+  __device__ __forceinline__ int runs() const { return rounds * width; }
+  __device__ __forceinline__ long base(int round) const { return rounds == 1 ? (round ? work : 0) : work * kShares[round] / 64; }
+  __device__ __forceinline__ long divide(long a, long b) const {  // both positive; 32 bits are much quicker
+    return (unsigned long)a >> 32 ? a / b : (long)((unsigned)a / (unsigned)b);
+  }
+  __device__ __forceinline__ long start(int run) const {
+    const int round = run / width, j = run - round * width;
+    const long b = base(round);
+    if (round == rounds) return work;
+    const long n = base(round + 1) - b, per = divide(n, width);
+    return b + j * per + min((long)j, n - per * width);
+  }
+  __device__ __forceinline__ int run_of(long chunk) const {
+    int round = 0;
+    while (round + 1 < rounds && base(round + 1) <= chunk) ++round;
+    const long b = base(round), n = base(round + 1) - b, per = divide(n, width), longer = n - per * width;
+    const long in = chunk - b, edge = longer * (per + 1);
+    return round * width + (int)(in < edge ? divide(in, per + 1) : longer + divide(in - edge, per));
+  }
+};
 
 struct DecodeArgs {
   const char* q;     // [batch][nq][D]
   char* out;         // [batch][nq][D], contiguous
   int* status;
-  float* parts;      // [ctas][2][kHeads][D + 2]: o, m, l
-  int4* joins;       // [ctas]: {first output row, heads, parts, -}: the item that starts in this CTA
+  float* parts;      // [runs][2][kHeads][D + 2]: o, m, l
+  int4* joins;       // [runs]: {first output row, heads, parts, -}: the item that starts in this run
                      // and ends in a later one; 0 parts where there is none
   long long q_row, q_head;
   int nq, rep, groups;  // groups of up to 8 query heads of a key head
+  int rounds;           // at the most
   float scale;          // scale * log2 e
 };
 
@@ -46,10 +84,8 @@ struct Ring {
   static constexpr int kHalves = D / 64;
   static constexpr uint32_t kBox = kChunk * 128;  // 64 elements of a chunk's rows
   static constexpr uint32_t kStage = 2 * kHalves * kBox;  // K and V
-  // an even number: a stage then belongs to one of the two groups of warps, which takes its phases
-  // one after the other (copies land out of order, and a parity tells only two phases apart)
-  static constexpr int kStages = D == 128 ? 6 : 12;
-  static constexpr uint32_t kMerge = kConsumers * kHeads * D * 4;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr uint32_t kMerge = (kConsumers - 1) * kHeads * D * 4;
   static constexpr uint32_t kBytes = kStages * kStage + kMerge + 1024;
 };
 
@@ -81,13 +117,13 @@ __device__ __forceinline__ uint32_t swizzled(int r, int piece) {
 // Chunks of a sequence; one even where it is empty, so that its rows get their zeros.
 __device__ __forceinline__ int chunks_of(int len) { return len > kChunk ? (len + kChunk - 1) / kChunk : 1; }
 
-// An item in a CTA's run: chunks [c0, c1) of sequence b for key head kh, query heads of `group`.
+// An item in a run: chunks [c0, c1) of sequence b for key head kh, query heads of `group`.
 struct Run {
   int b, kh, group, len, chunks, c0, c1;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kDecodeThreads, 1)
+__global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
     paged_decode(const __grid_constant__ DecodeArgs a, const __grid_constant__ Pages p,
                  const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using R = Ring<D>;
@@ -100,14 +136,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   volatile int* dead = &dead_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
-  float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp][head][D]
+  float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp - 1][head][D]
   long* slab = reinterpret_cast<long*>(merge);  // chunks (of one head) of the sequences before thread t's slab
 
   if (warp == kConsumers && lane < 2) prefetch_map(lane ? &vmap : &kmap);
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
+      mbar_init(&empty[i], kConsumers);
     }
     dead_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -137,14 +173,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   __syncthreads();
 
   const int per_seq = p.heads * a.groups;  // items of a sequence
-  const long work = total * per_seq;
-  // runs of equal length; no more of them than chunks, so that none between two others is empty
-  const long ctas = min((long)gridDim.x, work);
-  const long w0 = work * blockIdx.x / ctas, w1 = work * (blockIdx.x + 1) / ctas;
-  if (blockIdx.x >= ctas) {
-    if (tid == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+  const Plan plan(total * per_seq, gridDim.x, a.rounds);
+  const int run = blockIdx.x;
+  if (run >= plan.runs()) {
+    if (tid == 0) a.joins[run] = make_int4(0, 0, 0, 0);
     return;
   }
+  const long w0 = plan.start(run), w1 = plan.start(run + 1);
   // the sequence and item of chunk w0: every warp by itself
   Run r;
   long at = w0;  // the run's position in the flat order
@@ -166,7 +201,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     }
     r.b = b;
     const long in = w0 - before;
-    const int item = (int)(in / r.chunks);
+    const int item = (int)plan.divide(in, r.chunks);
     r.kh = item / a.groups;
     r.group = item - r.kh * a.groups;
     r.c0 = (int)(in - (long)item * r.chunks);
@@ -190,25 +225,31 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     return true;
   };
 
-  unsigned idx = 0;  // chunks of this CTA so far: stage idx % NS
+  unsigned idx = 0;  // chunks of this run so far: stage idx % NS
   if (warp == kConsumers) {
     // -------------------------------------------------------------------- loads
     bool ok = true;
-    const int rows = min(1 << p.shift, kChunk);  // of a box
+    const int rows = min(1 << p.shift, kChunk);           // of a box
+    const int per_chunk = kChunk / rows;                  // boxes of a chunk, for either half of K and of V
+    const int box = lane / (2 * R::kHalves), what = lane - box * 2 * R::kHalves;  // page, then half, K or V
     do {
       const int* table = p.table + r.b * p.table_row;
+      int ids = 0, first = 1 << 30;  // a lane a box: the page ids of the 32 boxes from `first` on
       for (int c = r.c0; c < r.c1; ++c, ++idx) {
         const unsigned st = idx % NS;
-        if (!(ok = !*dead && mbar_wait_bounded(&empty[st], ((idx / NS) & 1) ^ 1))) break;
         const int left = min(kChunk, r.len - c * kChunk), boxes = (left + rows - 1) / rows;
+        if (c * per_chunk < first || (c + 1) * per_chunk > first + 32) {
+          first = c * per_chunk;
+          const int key = (first + lane) * rows;
+          ids = key < r.len ? page_of(p, table, key, a.status) : 0;
+          if (ids < 0) ids = p.pages;  // out of range: the box reads as zeros
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, (c * per_chunk - first + box) & 31);
+        if (!(ok = !*dead && mbar_wait_bounded(&empty[st], ((idx / NS) & 1) ^ 1))) break;
         if (lane == 0) mbar_expect_tx(&full[st], boxes * rows * 128 * 2 * R::kHalves);
         __syncwarp();
-        // a lane a box: page, then half, then K or V
-        const int box = lane / (2 * R::kHalves), what = lane - box * 2 * R::kHalves;
         if (box < boxes) {
           const int key = c * kChunk + box * rows, hf = what % R::kHalves, v = what / R::kHalves;
-          int page = page_of(p, table, key, a.status);
-          if (page < 0) page = p.pages;  // out of range: the box reads as zeros
           tma_4d(ring + st * R::kStage + what * R::kBox + box * rows * 128, v ? &vmap : &kmap, hf * 64,
                  key & ((1 << p.shift) - 1), r.kh, page, &full[st]);
         }
@@ -225,7 +266,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 
   // ---------------------------------------------------------------------- attention
   const int g = lane >> 2, t4 = lane & 3;  // this lane's query head, and its keys 2 t4 (+1) of 8
-  const int tok0 = 16 * (warp & 3), side = warp >> 2;
+  const int tok0 = 16 * warp;
   do {
     const int heads = min(kHeads, a.rep - r.group * kHeads), row0 = r.b * a.nq + r.kh * a.rep + r.group * kHeads;
     uint32_t qa[NK][2];
@@ -238,7 +279,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     float o[2 * NK][4] = {};
     float m = -INFINITY, l = 0.f;  // of head g; l over this lane's keys
     for (int c = r.c0; c < r.c1; ++c, ++idx) {
-      if ((int)(idx & 1) != side) continue;
       const unsigned st = idx % NS;
       const int left = r.len - c * kChunk - tok0;  // keys of this warp's 16 and behind
       const bool got = !*dead && mbar_wait_bounded(&full[st], (idx / NS) & 1);
@@ -305,81 +345,113 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-    // the eight warps' parts of the item, joined through shared memory
+    // the warps' parts of the item: each brings its own to the common reference, warp 0 adds up
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t4 == 0) wm[warp][g] = m, wl[warp][g] = l;
-    float* mine_o = merge + (warp * kHeads + g) * D;
-#pragma unroll
-    for (int jd = 0; jd < 2 * NK; ++jd)
-      *reinterpret_cast<float2*>(mine_o + 8 * jd + 2 * t4) = make_float2(o[jd][0] + o[jd][2], o[jd][1] + o[jd][3]);
     pipe::named_sync(1, kConsumers * 32);
-    const bool whole = r.c0 == 0 && r.c1 == r.chunks;
-    float* part = a.parts + ((long long)blockIdx.x * 2 + (r.c0 == 0 ? 1 : 0)) * kHeads * (D + 2);
-    for (int e = tid; e < heads * (D / 2); e += kConsumers * 32) {
-      const int h = e / (D / 2), d = 2 * (e - h * (D / 2));
-      float mm = -INFINITY;
+    float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < kConsumers; ++w) mm = fmaxf(mm, wm[w][h]);
-      const float ref = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int w = 0; w < kConsumers; ++w) mm = fmaxf(mm, wm[w][g]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-      for (int w = 0; w < kConsumers; ++w) {
-        const float f = ex2(wm[w][h] - ref);
-        const float2 v = *reinterpret_cast<const float2*>(merge + (w * kHeads + h) * D + d);
-        ll = fmaf(f, wl[w][h], ll);
-        x0 = fmaf(f, v.x, x0);
-        x1 = fmaf(f, v.y, x1);
-      }
-      if (whole) {
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        *reinterpret_cast<uint32_t*>(a.out + ((long long)(row0 + h) * D + d) * 2) = Elem<T>::pack(x0 * inv, x1 * inv);
-      } else {
-        *reinterpret_cast<float2*>(part + h * D + d) = make_float2(x0, x1);
-        if (d == 0) part[kHeads * D + h] = mm, part[kHeads * D + kHeads + h] = ll;
-      }
+    for (int w = 0; w < kConsumers; ++w) ll = fmaf(ex2(wm[w][g] - ref), wl[w][g], ll);
+    const float f = ex2(m - ref);
+    if (warp) {
+      float* mine_o = merge + ((warp - 1) * kHeads + g) * D;
+#pragma unroll
+      for (int jd = 0; jd < 2 * NK; ++jd)
+        *reinterpret_cast<float2*>(mine_o + 8 * jd + 2 * t4) =
+            make_float2((o[jd][0] + o[jd][2]) * f, (o[jd][1] + o[jd][3]) * f);
     }
-    if (tid == 0 && at + (r.c1 - r.c0) >= w1) {  // this CTA's last item: does it go on in the next ones?
-      int n = 0;
-      if (r.c0 == 0 && r.c1 < r.chunks) {
-        const long end = at + r.chunks;  // its end in the flat order
-        n = 2;
-        while (work * (blockIdx.x + n) / ctas < end) ++n;
+    pipe::named_sync(1, kConsumers * 32);
+    if (warp == 0) {
+      const bool whole = r.c0 == 0 && r.c1 == r.chunks;
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      float* part = a.parts + ((long long)run * 2 + (r.c0 == 0 ? 1 : 0)) * kHeads * (D + 2);
+#pragma unroll
+      for (int jd = 0; jd < 2 * NK; ++jd) {
+        const int d = 8 * jd + 2 * t4;
+        float x0 = (o[jd][0] + o[jd][2]) * f, x1 = (o[jd][1] + o[jd][3]) * f;
+#pragma unroll
+        for (int w = 0; w < kConsumers - 1; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(merge + (w * kHeads + g) * D + d);
+          x0 += v.x;
+          x1 += v.y;
+        }
+        if (g < heads) {
+          if (whole)
+            *reinterpret_cast<uint32_t*>(a.out + ((long long)(row0 + g) * D + d) * 2) = Elem<T>::pack(x0 * inv, x1 * inv);
+          else
+            *reinterpret_cast<float2*>(part + g * D + d) = make_float2(x0, x1);
+        }
       }
-      a.joins[blockIdx.x] = make_int4(row0, heads, n, 0);
+      if (!whole && t4 == 0) part[kHeads * D + g] = mm, part[kHeads * D + kHeads + g] = ll;
+      if (lane == 0 && at + (r.c1 - r.c0) >= w1)  // the run's last item: does it go on in the next ones?
+        a.joins[run] = make_int4(row0, heads,
+                                 r.c0 == 0 && r.c1 < r.chunks ? plan.run_of(at + r.chunks - 1) - run + 1 : 0, 0);
     }
     pipe::named_sync(1, kConsumers * 32);
   } while (advance());
 }
 
-// Joins the parts of the items that more than one CTA worked on: block (c, h) the item that starts in
-// CTA c's run, query head h of its group.
+// Joins the parts of the items that more than one run worked on: block column c the item that starts in
+// run c. With a block row a query head, the block's warps take a share of the parts each (few items of
+// many parts); with one row they take a head each (many items of two parts).
+constexpr int kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(D) paged_decode_join(const __grid_constant__ DecodeArgs a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_decode_join(const __grid_constant__ DecodeArgs a) {
+  constexpr int E = D / 32;
+  __shared__ float ol[kJoinWarps], oo[kJoinWarps][D];
   pdl_wait();
-  const int c = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 j = a.joins[c];
-  if (h >= j.y || j.z == 0) return;
-  auto part = [&](int i) {  // its first part in slot 1 of CTA c, the others in slot 0 of the next ones
+  if (j.z == 0) return;
+  const bool shared = gridDim.y > 1;
+  const int first = shared ? warp : 0, stride = shared ? kJoinWarps : 1;
+  auto part = [&](int i) {  // the first in slot 1 of run c, the others in slot 0 of the next ones
     return a.parts + ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * kHeads * (D + 2);
   };
-  float m = -INFINITY;
-  for (int i = 0; i < j.z; ++i) m = fmaxf(m, part(i)[kHeads * D + h]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  for (int i = 0; i < j.z; ++i) {
-    const float* x = part(i);
-    const float f = ex2(x[kHeads * D + h] - ref);
-    l = fmaf(f, x[kHeads * D + kHeads + h], l);
-    o = fmaf(f, x[h * D + d], o);
+  for (int h = shared ? blockIdx.y : warp; h < j.y; h += shared ? gridDim.y : kJoinWarps) {
+    float m = -INFINITY;
+    for (int i = lane; i < j.z; i += 32) m = fmaxf(m, part(i)[kHeads * D + h]);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[E] = {};
+#pragma unroll 8
+    for (int i = first; i < j.z; i += stride) {
+      const float* x = part(i);
+      const float f = ex2(x[kHeads * D + h] - ref);
+      l = fmaf(f, x[kHeads * D + kHeads + h], l);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(x + h * D + lane * E + e);
+        o[e] = fmaf(f, v.x, o[e]);
+        o[e + 1] = fmaf(f, v.y, o[e + 1]);
+      }
+    }
+    if (shared) {
+      if (lane == 0) ol[warp] = l;
+#pragma unroll
+      for (int e = 0; e < E; ++e) oo[warp][lane * E + e] = o[e];
+      __syncthreads();
+      if (warp) return;
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w) {
+        l += ol[w];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += oo[w][lane * E + e];
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)(j.x + h) * D + lane * E) * 2);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
   }
-  const float v = o * (l == 0.f ? 0.f : 1.f / l);
-  const uint32_t w = Elem<T>::pack(v, 0.f);
-  *reinterpret_cast<uint16_t*>(a.out + ((long long)(j.x + h) * D + d) * 2) = (uint16_t)w;
 }
 
 template <typename T, int D>
-static cudaError_t launch_decode(const DecodeArgs& a, const Pages& p, int ctas, cudaStream_t s, int flags) {
+static cudaError_t launch_decode(const DecodeArgs& a, const Pages& p, int runs, cudaStream_t s, int flags) {
   constexpr bool fp16 = __is_same(T, __half);
   CUtensorMap km, vm;
   const cuuint64_t page = 1ull << p.shift;
@@ -389,15 +461,17 @@ static cudaError_t launch_decode(const DecodeArgs& a, const Pages& p, int ctas, 
   const cuuint32_t box[4] = {64, (cuuint32_t)(page < kChunk ? page : kChunk), 1, 1};
   if (!tensor_map(&km, fp16, 4, p.k, d, ks, box) || !tensor_map(&vm, fp16, 4, p.v, d, vs, box))
     return cudaErrorInvalidValue;
-  cudaError_t e = launch(paged_decode<T, D>, dim3(ctas), dim3(kDecodeThreads), Ring<D>::kBytes, s, flags, a, p, km, vm);
+  cudaError_t e = launch(paged_decode<T, D>, dim3(runs), dim3(kDecodeThreads), Ring<D>::kBytes, s, flags, a, p, km, vm);
   if (e != cudaSuccess) return e;
-  return launch(paged_decode_join<T, D>, dim3(ctas, kHeads), dim3(D), 0, s, flags | kFlagPdl, a);
+  return launch(paged_decode_join<T, D>, dim3(runs, a.rounds > 1 ? 1 : kHeads), dim3(32 * kJoinWarps), 0, s,
+                flags | kFlagPdl, a);
 }
 
-// CTAs of a call: one an SM, no more than there can be chunks.
-static int decode_ctas(int batch, int heads, int groups, long long max_len) {
-  const long long most = (long long)batch * heads * groups * ((max_len + kChunk - 1) / kChunk);
-  return (int)(most < sm_count() ? most : sm_count());
+// Rounds of a call: more than one where the items alone, or the lengths that the page table allows, give
+// every resident CTA plenty to do.
+static int rounds_of(long long items, long long most_chunks) {
+  const long long resident = (long long)kCtasPerSm * sm_count();
+  return items >= 2 * resident || most_chunks >= 64 * resident ? kRounds : 1;
 }
 
 }  // namespace paged
@@ -421,7 +495,8 @@ using namespace mt;
 // Workspace bytes of mt_paged_attention_decode on the current device, whatever the sizes.
 MT_API int mt_paged_attention_decode_workspace(long long* bytes) {
   if (!bytes) return kBadArgument;
-  *bytes = (long long)sm_count() * (2 * paged::kHeads * (128 + 2) * sizeof(float) + sizeof(int4));
+  const long long runs = (long long)paged::kRounds * paged::kCtasPerSm * sm_count();
+  *bytes = runs * (2 * paged::kHeads * (128 + 2) * sizeof(float) + sizeof(int4));
   return 0;
 }
 
@@ -435,14 +510,17 @@ MT_API int mt_paged_attention_decode(const void* q, int q_row, int q_head, const
       !aligned(workspace, 16))
     return kBadArgument;
   const int rep = nq / kv->heads, groups = (rep + paged::kHeads - 1) / paged::kHeads;
-  const int ctas = paged::decode_ctas(kv->batch, kv->heads, groups, (long long)kv->max_pages * kv->page_size);
+  const long long items = (long long)kv->batch * kv->heads * groups;
+  const long long most = items * (((long long)kv->max_pages * kv->page_size + paged::kChunk - 1) / paged::kChunk);
+  const long long resident = (long long)paged::kCtasPerSm * sm_count();
+  const int rounds = paged::rounds_of(items, most), runs = (int)(rounds > 1 ? rounds * resident : most < resident ? most : resident);
   int4* joins = (int4*)workspace;
-  const paged::DecodeArgs a{(const char*)q, (char*)out, (int*)status, (float*)(joins + sm_count()), joins, q_row, q_head,
-                            nq, rep, groups, scale * paged::kLog2e};
+  const paged::DecodeArgs a{(const char*)q, (char*)out, (int*)status, (float*)(joins + paged::kRounds * resident), joins,
+                            q_row, q_head, nq, rep, groups, rounds, scale * paged::kLog2e};
   const cudaStream_t s = (cudaStream_t)stream;
   if (kv->type == 0)
-    return kv->head_dim == 128 ? paged::launch_decode<__nv_bfloat16, 128>(a, p, ctas, s, flags)
-                               : paged::launch_decode<__nv_bfloat16, 64>(a, p, ctas, s, flags);
-  return kv->head_dim == 128 ? paged::launch_decode<__half, 128>(a, p, ctas, s, flags)
-                             : paged::launch_decode<__half, 64>(a, p, ctas, s, flags);
+    return kv->head_dim == 128 ? paged::launch_decode<__nv_bfloat16, 128>(a, p, runs, s, flags)
+                               : paged::launch_decode<__nv_bfloat16, 64>(a, p, runs, s, flags);
+  return kv->head_dim == 128 ? paged::launch_decode<__half, 128>(a, p, runs, s, flags)
+                             : paged::launch_decode<__half, 64>(a, p, runs, s, flags);
 }
