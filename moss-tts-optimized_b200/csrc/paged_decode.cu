@@ -85,7 +85,8 @@ struct Ring {
   static constexpr uint32_t kBox = kChunk * 128;  // 64 elements of a chunk's rows
   static constexpr uint32_t kStage = 2 * kHalves * kBox;  // K and V
   static constexpr int kStages = D == 128 ? 3 : 6;
-  static constexpr uint32_t kMerge = (kConsumers - 1) * kHeads * D * 4;
+  static constexpr int kRow = D + 8;  // floats of a merge row: the eight heads on banks of their own
+  static constexpr uint32_t kMerge = (kConsumers - 1) * kHeads * kRow * 4;
   static constexpr uint32_t kBytes = kStages * kStage + kMerge + 1024;
 };
 
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
   volatile int* dead = &dead_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t ring = (smem_u32(raw) + 1023) & ~1023u;
-  float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp - 1][head][D]
+  float* merge = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)) + NS * R::kStage);  // [warp - 1][head][kRow]
   long* slab = reinterpret_cast<long*>(merge);  // chunks (of one head) of the sequences before thread t's slab
 
   if (warp == kConsumers && lane < 2) prefetch_map(lane ? &vmap : &kmap);
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
     for (int w = 0; w < kConsumers; ++w) ll = fmaf(ex2(wm[w][g] - ref), wl[w][g], ll);
     const float f = ex2(m - ref);
     if (warp) {
-      float* mine_o = merge + ((warp - 1) * kHeads + g) * D;
+      float* mine_o = merge + ((warp - 1) * kHeads + g) * R::kRow;
 #pragma unroll
       for (int jd = 0; jd < 2 * NK; ++jd)
         *reinterpret_cast<float2*>(mine_o + 8 * jd + 2 * t4) =
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
         float x0 = (o[jd][0] + o[jd][2]) * f, x1 = (o[jd][1] + o[jd][3]) * f;
 #pragma unroll
         for (int w = 0; w < kConsumers - 1; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(merge + (w * kHeads + g) * D + d);
+          const float2 v = *reinterpret_cast<const float2*>(merge + (w * kHeads + g) * R::kRow + d);
           x0 += v.x;
           x1 += v.y;
         }
@@ -402,7 +403,8 @@ constexpr int kJoinWarps = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_decode_join(const __grid_constant__ DecodeArgs a) {
   constexpr int E = D / 32;
-  __shared__ float ol[kJoinWarps], oo[kJoinWarps][D];
+  __shared__ float om[kJoinWarps], ol[kJoinWarps], oo[kJoinWarps][D];
+  static_assert(kJoinWarps == 4, "the maximum below");
   pdl_wait();
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 j = a.joins[c];
@@ -413,34 +415,56 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_decode_join(const __gri
     return a.parts + ((long long)(c + i) * 2 + (i == 0 ? 1 : 0)) * kHeads * (D + 2);
   };
   for (int h = shared ? blockIdx.y : warp; h < j.y; h += shared ? gridDim.y : kJoinWarps) {
-    float m = -INFINITY;
-    for (int i = lane; i < j.z; i += 32) m = fmaxf(m, part(i)[kHeads * D + h]);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[E] = {};
-#pragma unroll 8
-    for (int i = first; i < j.z; i += stride) {
-      const float* x = part(i);
-      const float f = ex2(x[kHeads * D + h] - ref);
-      l = fmaf(f, x[kHeads * D + kHeads + h], l);
+    // eight parts at a time, all their loads under way at once
+    float m = -INFINITY, l = 0.f, o[E] = {};
+    for (int i0 = first; i0 < j.z; i0 += 8 * stride) {
+      float pm[8], pl[8], po[8][E], top = m;
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(x + h * D + lane * E + e);
-        o[e] = fmaf(f, v.x, o[e]);
-        o[e + 1] = fmaf(f, v.y, o[e + 1]);
+      for (int n = 0; n < 8; ++n) {
+        const int i = i0 + n * stride;
+        pm[n] = -INFINITY;
+        if (i < j.z) {
+          const float* x = part(i);
+          pm[n] = x[kHeads * D + h], pl[n] = x[kHeads * D + kHeads + h];
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(x + h * D + lane * E + e);
+            po[n][e] = v.x, po[n][e + 1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) top = fmaxf(top, pm[n]);
+      const float ref = top == -INFINITY ? 0.f : top, keep = ex2(m - ref);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= keep;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        if (i0 + n * stride >= j.z) continue;
+        const float f = ex2(pm[n] - ref);
+        l = fmaf(f, pl[n], l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(f, po[n][e], o[e]);
       }
     }
     if (shared) {
-      if (lane == 0) ol[warp] = l;
+      if (lane == 0) om[warp] = m, ol[warp] = l;
 #pragma unroll
       for (int e = 0; e < E; ++e) oo[warp][lane * E + e] = o[e];
       __syncthreads();
       if (warp) return;
+      const float top = fmaxf(fmaxf(om[0], om[1]), fmaxf(om[2], om[3])), ref = top == -INFINITY ? 0.f : top;
+      l = 0.f;
 #pragma unroll
-      for (int w = 1; w < kJoinWarps; ++w) {
-        l += ol[w];
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += oo[w][lane * E + e];
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = ex2(om[w] - ref);
+        l = fmaf(f, ol[w], l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(f, oo[w][lane * E + e], o[e]);
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
