@@ -1,5 +1,5 @@
 // Shared pieces of the paged key-value cache's kernels (sm_100a): 16-bit element types, where a
-// key's row lies (in pages or packed), which sequence a packed token belongs to, and the attention
+// key's row lies (in pages or packed), which sequence a packed token belongs to, packed fp32 arithmetic, and the attention
 // of one query row by one warp.
 #pragma once
 #include <cuda_fp16.h>
@@ -33,6 +33,24 @@ struct Elem<__half> {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 };
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 
 // One layer's pages, as mt_paged_kv with the element strides of a page, a head and a row.
 struct Pages {

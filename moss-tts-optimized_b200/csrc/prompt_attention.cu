@@ -25,7 +25,9 @@ namespace mt {
 namespace prompt {
 
 using namespace tcore;
+using paged::add2;
 using paged::Elem;
+using paged::fma2;
 using paged::Pages;
 using pipe::mbar_arrive;
 using pipe::mbar_expect_tx;

@@ -1,4 +1,4 @@
-// tcgen05, TMA and packed-fp32 primitives of the prompt attention (sm_100a).
+// tcgen05 and TMA primitives of the paged cache's attention (sm_100a).
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -153,23 +153,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
-      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
-      " mov.b64 {%0, %1}, d;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // Host: a tensor map of 16-bit elements, boxes with the 128-byte swizzle; dims, strides (bytes, of
 // dims 1..) and box sizes innermost first. Out-of-range elements read as zeros.
 static inline bool tensor_map(CUtensorMap* map, bool fp16, int rank, const void* base, const cuuint64_t* dims,
