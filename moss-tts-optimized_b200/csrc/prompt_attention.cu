@@ -56,6 +56,7 @@ struct Reference {
   static constexpr float most = kChecked ? 256.f : 1073741824.f, fits = 32768.f;
 };
 
+struct Joined;
 struct PromptArgs {
   const char* q;     // [tokens_q][nq][D]
   const char *k, *v; // [tokens_k][nkv][D] (packed form)
@@ -66,10 +67,12 @@ struct PromptArgs {
   int tokens_q, tokens_k, batch, nq, nkv, rep, causal;
   int tok;           // tokens of a query tile: 128 / rep
   float scale;       // scale * log2 e
-  // where items may be cut along their keys: the most pieces there may be, and per piece
-  // [256 rows][D] unnormalised outputs, [256] references, [256] sums
+  // where items may be cut along their keys: the most pieces there may be; per piece unnormalised outputs
+  // [D / 8][256 rows][8] (a warp's 32 rows store whole lines), [256] references, [256] sums; and every
+  // item's place for the join
   int units;
   float* parts;
+  Joined* joined;
 };
 
 // Rows [first, first + n) of sequence b in a packed buffer of `tokens` rows; offsets outside the
@@ -95,8 +98,18 @@ __device__ __forceinline__ int keys_seen(const PromptArgs& a, const Item& it, in
   return a.causal ? min(max(it.len - it.lq + t + 1, 0), it.len) : it.len;
 }
 
+struct __align__(16) Joined {  // an item and the pieces it is cut into; 0 pieces: no such item
+  Item it;
+  int cut, pad[3];
+};
+
 // Tile pairs of a sequence of lq new tokens.
 __device__ __forceinline__ int pairs_of(const PromptArgs& a, int lq) { return (lq + 2 * a.tok - 1) / (2 * a.tok); }
+
+// The most items that a call can have, whatever its sequences' lengths.
+__host__ __device__ __forceinline__ long long items_most(const PromptArgs& a) {
+  return ((long long)a.tokens_q / (2 * a.tok) + a.batch) * a.nkv;
+}
 
 // Finds flat item w = (query tile pair, key head); pairs in order of the sequences and, inside one,
 // from its end, where a causal row sees most. By a converged warp; rising indices are found without a new
@@ -151,8 +164,7 @@ struct Finder {
 // the workspace and a join, about two tiles). By a converged warp.
 template <bool PAGED>
 __device__ int pieces(const PromptArgs& a, const Pages& p, int lane) {
-  long pairs = 0;
-  int longest = 0;
+  int pairs = 0, longest = 0;  // pieces are cut where there are few pairs: 32 bits hold everything here
   for (int b = lane; b < a.batch; b += 32) {
     int first, lq, len;
     span_of(a.cu_q, b, a.tokens_q, first, lq);
@@ -163,13 +175,9 @@ __device__ int pieces(const PromptArgs& a, const Pages& p, int lane) {
     pairs += pairs_of(a, lq);
     if (lq) longest = max(longest, len);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  const long items = max(pairs * a.nkv, 1L);
-  return (int)max(1L, min(a.units / items, (long)(tiles_of(longest) / 3)));
+  pairs = __reduce_add_sync(0xffffffffu, pairs);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  return max(1, min(a.units / max(pairs * a.nkv, 1), tiles_of(longest) / 3));
 }
 
 // Waits for a phase. Where that does not come, the kernel gives up: `dead` ends this and every later
@@ -479,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (live) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              store32(part + r * D + 32 * c + 8 * e, reinterpret_cast<const uint32_t(&)[8]>(ow[8 * e]));
+              store32(part + ((4 * c + e) * (2 * kTile) + r) * 8, reinterpret_cast<const uint32_t(&)[8]>(ow[8 * e]));
           }
         }
         continue;
@@ -709,12 +717,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (SPLIT) {
         if (n) wait_for(&item_empty, (n - 1) & 1, dead);
         const int piece = blockIdx.x - w * cut, tiles = it.j1;
-        it.j0 = (int)((long)tiles * piece / cut);
-        it.j1 = (int)((long)tiles * (piece + 1) / cut);
+        it.j0 = (int)((unsigned)(tiles * piece) / (unsigned)cut);  // at most 2^23 tiles x 148 pieces
+        it.j1 = (int)((unsigned)(tiles * (piece + 1)) / (unsigned)cut);
       }
       if (lane == 0) {
         item_s = it;
         mbar_arrive(&item_full);
+      }
+      if (SPLIT && n == 0 && blockIdx.x < items_most(a)) {  // beside it, this block's share of the list for the join
+        Finder all;
+        Joined* j = a.joined + blockIdx.x;
+        Item listed;
+        const bool there = all.find<PAGED>(a, p, lane, blockIdx.x, listed);
+        if (lane == 0) {
+          if (there) j->it = listed;
+          j->cut = there ? cut : 0;
+        }
       }
       if (it.none) break;
     }
@@ -729,58 +747,82 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the items, a warp a row:  m = max m_i,
-// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i, pieces in the order of the keys.
+// Joins the pieces of the items, a warp a row; D/8 lanes (32 bytes each) take one piece, the other lanes
+// the next:  m = max m_i,
+// o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
 constexpr int kJoinRows = 8;  // of a block
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(32 * kJoinRows) prompt_join(const __grid_constant__ PromptArgs a, const __grid_constant__ Pages p) {
-  constexpr int E = D / 32;
+  constexpr int kLanes = D / 8, kGroups = 32 / kLanes, kAtOnce = 8;
   pdl_wait();
   const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
-  const int cut = pieces<PAGED>(a, p, lane), tile = r / kTile, rtok = (r % kTile) / a.rep, rhead = r % kTile - rtok * a.rep;
-  Finder finder;
-  Item it;
-  if (!finder.find<PAGED>(a, p, lane, blockIdx.x, it)) return;  // one block column an item
+  const int cut = a.joined[blockIdx.x].cut;
+  const Item it = a.joined[blockIdx.x].it;
+  const int tile = r / kTile, rtok = (r % kTile) / a.rep, rhead = r % kTile - rtok * a.rep;
   const int t = it.t0 + tile * a.tok + rtok;
-  if (rtok >= a.tok || t >= it.lq) return;
+  if (cut == 0 || rtok >= a.tok || t >= it.lq) return;
   const int h = it.kh * a.rep + rhead, seen = keys_seen(a, it, t);
   const float* part = a.parts + (long long)blockIdx.x * cut * (2 * kTile) * (D + 2);
-  auto at = [&](int i) { return part + (long long)i * (2 * kTile) * (D + 2); };
-  float m = -INFINITY;
-  for (int i = lane; i < cut; i += 32) m = fmaxf(m, at(i)[2 * kTile * D + r]);
-  m = warp_max(m);
-  float l = 0.f, o[E] = {};
-  for (int i = 0; i < cut; ++i) {
-    const float mi = at(i)[2 * kTile * D + r];
-    if (mi == -INFINITY) continue;
-    const float f = ex2(mi - m);
-    l = fmaf(f, at(i)[2 * kTile * (D + 1) + r], l);
-    const float* x = at(i) + r * D + lane * E;
+  const int sub = lane / kLanes, d8 = lane - sub * kLanes;
+  // eight pieces at a time and group of lanes, all their loads under way at once
+  float m = -INFINITY, l = 0.f, o[8] = {};
+  for (int i0 = sub; i0 < cut; i0 += kAtOnce * kGroups) {
+    float pm[kAtOnce], pl[kAtOnce], top = m;
+    float4 po[kAtOnce][2];
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(x + e);
-      o[e] = fmaf(f, v.x, o[e]);
-      o[e + 1] = fmaf(f, v.y, o[e + 1]);
+    for (int n = 0; n < kAtOnce; ++n) {
+      pm[n] = -INFINITY;
+      if (i0 + n * kGroups < cut) {
+        const float* x = part + (long long)(i0 + n * kGroups) * (2 * kTile) * (D + 2);
+        const float4* y = reinterpret_cast<const float4*>(x + (d8 * (2 * kTile) + r) * 8);
+        pm[n] = x[2 * kTile * D + r], pl[n] = x[2 * kTile * (D + 1) + r];
+        po[n][0] = y[0], po[n][1] = y[1];
+      }
     }
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) top = fmaxf(top, pm[n]);
+    const float ref = top == -INFINITY ? 0.f : top, keep = ex2(m - ref);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= keep;
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      if (pm[n] == -INFINITY) continue;  // no key there: nothing was written
+      const float f = ex2(pm[n] - ref);
+      const float* v = reinterpret_cast<const float*>(po[n]);
+      l = fmaf(f, pl[n], l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(f, v[e], o[e]);
+    }
+  }
+#pragma unroll
+  for (int x = kLanes; x < 32; x <<= 1) {  // the groups of lanes
+    const float om = __shfl_xor_sync(0xffffffffu, m, x), top = fmaxf(m, om), ref = top == -INFINITY ? 0.f : top;
+    const float f = ex2(m - ref), of = ex2(om - ref);
+    l = l * f + __shfl_xor_sync(0xffffffffu, l, x) * of;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = o[e] * f + __shfl_xor_sync(0xffffffffu, o[e], x) * of;
+    m = top;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float odd = 0.f;
+  uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    o[e] *= inv;
-    odd = fmaf(o[e], 0.f, odd);
+  for (int e = 0; e < 4; ++e) {
+    const float x = o[2 * e] * inv, y = o[2 * e + 1] * inv;
+    odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
+    w[e] = Elem<T>::pack(x, y);
   }
   if (__any_sync(0xffffffffu, !(odd == 0.f))) {
     row_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, seen, it.q0 + t, h);
     return;
   }
-  uint32_t* op = reinterpret_cast<uint32_t*>(a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2) + lane * (E / 2);
-#pragma unroll
-  for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e], o[2 * e + 1]);
+  if (sub == 0)
+    *reinterpret_cast<uint4*>(a.out + (((long long)(it.q0 + t) * a.nq + h) * D + d8 * 8) * 2) =
+        make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The most items that a call can have, whatever its sequences' lengths.
-static long long items_most(const PromptArgs& a) { return ((long long)a.tokens_q / (2 * a.tok) + a.batch) * a.nkv; }
 // Query map: boxes of 64 elements x rep heads x 128 / rep tokens. Keys and values: 64 elements x up to
 // 128 rows of one head, of a page or of the packed rows.
 template <typename T, int D, bool PAGED>
@@ -830,7 +872,13 @@ static cudaError_t launch_prompt(const PromptArgs& a, const Pages& p, int d, int
 // enough for two pieces (six tiles).
 static long long workspace_of(const PromptArgs& a, long long keys, int d) {
   if (2 * items_most(a) > sm_count() || keys <= 5 * kTile) return 0;
-  return (long long)sm_count() * (2 * kTile) * (d + 2) * sizeof(float);
+  return (long long)sm_count() * ((2 * kTile) * (d + 2) * sizeof(float) + sizeof(Joined));
+}
+
+static void cut_items(PromptArgs* a, void* workspace, int d) {
+  if (!workspace) return;
+  a->parts = (float*)workspace;
+  a->joined = (Joined*)(a->parts + (long long)a->units * (2 * kTile) * (d + 2));
 }
 
 static bool query_ok(const void* q, int q_row, int q_head, const void* cu, int tokens, int nq, int nkv, const void* out) {
@@ -880,8 +928,8 @@ MT_API int mt_packed_attention(const void* q, int q_row, int q_head, const void*
   prompt::PromptArgs a{(const char*)q, (const char*)k, (const char*)v, (char*)out, (const int*)cu_q,
                        (const int*)cu_k, nullptr, q_row, q_head, k_row, k_head, v_row, v_head,
                        tokens_q, tokens_k, batch, nq, nkv, rep, causal != 0, prompt::kTile / rep,
-                       scale * paged::kLog2e, sm_count(), nullptr};
-  if (workspace && prompt::workspace_of(a, tokens_k, head_dim)) a.parts = (float*)workspace;
+                       scale * paged::kLog2e, sm_count(), nullptr, nullptr};
+  if (prompt::workspace_of(a, tokens_k, head_dim)) prompt::cut_items(&a, workspace, head_dim);
   return prompt::launch_prompt<false>(a, paged::Pages{}, head_dim, type, (cudaStream_t)stream, flags);
 }
 
@@ -896,7 +944,8 @@ MT_API int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const
   const int rep = nq / kv->heads;
   prompt::PromptArgs a{(const char*)q, nullptr, nullptr, (char*)out, (const int*)cu_seqlens, nullptr, (int*)status,
                        q_row, q_head, 0, 0, 0, 0, tokens, 0, kv->batch, nq, kv->heads, rep, 1,
-                       prompt::kTile / rep, scale * paged::kLog2e, sm_count(), nullptr};
-  if (workspace && prompt::workspace_of(a, (long long)kv->max_pages * kv->page_size, kv->head_dim)) a.parts = (float*)workspace;
+                       prompt::kTile / rep, scale * paged::kLog2e, sm_count(), nullptr, nullptr};
+  if (prompt::workspace_of(a, (long long)kv->max_pages * kv->page_size, kv->head_dim))
+    prompt::cut_items(&a, workspace, kv->head_dim);
   return prompt::launch_prompt<true>(a, p, kv->head_dim, kv->type, (cudaStream_t)stream, flags);
 }
