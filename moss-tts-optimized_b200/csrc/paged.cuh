@@ -108,36 +108,50 @@ template <typename T, int D, typename Rows>
 __device__ __forceinline__ void row_attention(const float (&q)[D / 32], int n, int lane, Rows rows,
                                               float (&o)[D / 32]) {
   constexpr int E = D / 32;
+  constexpr int kAtOnce = 4;  // keys whose rows are on their way at once
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int j = 0; j < n; ++j) {
-    const T *kr, *vr;
-    rows(j, kr, vr);
-    uint32_t kw[E / 2] = {}, vw[E / 2] = {};
-    if (kr) {
+  for (int j0 = 0; j0 < n; j0 += kAtOnce) {
+    uint32_t kw[kAtOnce][E / 2], vw[kAtOnce][E / 2];
+    float s[kAtOnce], mn = m;
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      const T *kr = nullptr, *vr = nullptr;
+      if (j0 + x < n) rows(j0 + x, kr, vr);
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
-        kw[e] = reinterpret_cast<const uint32_t*>(kr)[lane * (E / 2) + e];
-        vw[e] = reinterpret_cast<const uint32_t*>(vr)[lane * (E / 2) + e];
+        kw[x][e] = kr ? reinterpret_cast<const uint32_t*>(kr)[lane * (E / 2) + e] : 0u;
+        vw[x][e] = vr ? reinterpret_cast<const uint32_t*>(vr)[lane * (E / 2) + e] : 0u;
       }
     }
-    float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float2 kf = Elem<T>::unpack(kw[e]);
-      s = fmaf(q[2 * e], kf.x, fmaf(q[2 * e + 1], kf.y, s));
+    for (int x = 0; x < kAtOnce; ++x) {
+      s[x] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        const float2 kf = Elem<T>::unpack(kw[x][e]);
+        s[x] = fmaf(q[2 * e], kf.x, fmaf(q[2 * e + 1], kf.y, s[x]));
+      }
+      s[x] = warp_sum(s[x]);
+      if (j0 + x >= n) s[x] = -INFINITY;
+      mn = fmaxf(mn, s[x]);
     }
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float keep = exp2f(m - ref), p = exp2f(s - ref);
+    const float ref = mn == -INFINITY ? 0.f : mn, keep = exp2f(m - ref);
     m = mn;
-    l = l * keep + p;
+    l *= keep;
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float2 vf = Elem<T>::unpack(vw[e]);
-      o[2 * e] = fmaf(p, vf.x, o[2 * e] * keep);
-      o[2 * e + 1] = fmaf(p, vf.y, o[2 * e + 1] * keep);
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      const float p = exp2f(s[x] - ref);
+      l += p;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) {
+        const float2 vf = Elem<T>::unpack(vw[x][e]);
+        o[2 * e] = fmaf(p, vf.x, o[2 * e]);
+        o[2 * e + 1] = fmaf(p, vf.y, o[2 * e + 1]);
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;

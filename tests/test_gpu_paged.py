@@ -259,6 +259,66 @@ def test_packed_rising_scores_move_the_running_maximum(cuda_device):
         check(f"rising by {sign}", got, want, bound)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 64), (HF, 128)])
+@pytest.mark.parametrize("step", [0.125, 0.02, -0.125])
+def test_packed_rising_scores_in_either_type(cuda_device, dtype, d, step):
+    """Steps whose weights leave fp16's range, or the reference's, by little and by far."""
+    dev, n = cuda_device, 500
+    q = torch.ones(n, 2, d, device=dev, dtype=dtype)
+    k = (torch.arange(n, device=dev)[:, None, None] * step).expand(n, 2, d).to(dtype).contiguous()
+    v = normal(75, n, 2, d, dtype=dtype, device=dev)
+    got = K.packed_attention(q, k, v, offsets([n], dev))
+    want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], d ** -0.5, True, dtype, UNIT[dtype])
+    check(f"rising by {step} {dtype}", got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("first", [12.0, -12.0])
+def test_packed_first_key_far_from_the_others(cuda_device, dtype, first):
+    """The reference starts at the first key's score: here scores of +-136 beside some of +-10."""
+    dev, n, d = cuda_device, 300, 128
+    q = torch.ones(n, 2, d, device=dev, dtype=dtype)
+    k = normal(76, n, 2, d, dtype=dtype, device=dev)
+    k[0] = first
+    v = normal(77, n, 2, d, dtype=dtype, device=dev)
+    got = K.packed_attention(q, k, v, offsets([n], dev))
+    want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], d ** -0.5, True, dtype, UNIT[dtype])
+    check(f"first key {first} {dtype}", got, want, bound)
+
+
+def test_packed_many_short_sequences(cuda_device):
+    """More items than CTAs, taken on demand, among them empty sequences."""
+    r = np.random.default_rng(78)
+    new = [int(x) for x in r.integers(0, 30, 900)]
+    _packed(cuda_device, 79, new, [n + int(x) for n, x in zip(new, r.integers(0, 40, 900))], 4, 2, 64, BF, pad=5)
+    _packed(cuda_device, 79, new[:300], new[:300], 6, 3, 128, HF)
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,d", [(BF, 4, 1, 128), (HF, 6, 2, 64), (BF, 14, 2, 64), (HF, 8, 1, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_rows_over_many_keys_are_cut_and_joined(cuda_device, dtype, nq, nkv, d, causal):
+    _packed(cuda_device, 200, [48], [4097], nq, nkv, d, dtype, causal=causal, pad=2)
+    _packed(cuda_device, 201, [1, 0, 3], [2500, 700, 0], nq, nkv, d, dtype, causal=causal)
+    _packed(cuda_device, 202, [40, 2], [30, 1700], nq, nkv, d, dtype, causal=causal)  # rows without a key
+
+
+def test_cut_prompts_over_pages(cuda_device):
+    dev, nq, nkv, d, page = cuda_device, 8, 2, 128, 32
+    new, lens = [20, 1, 0], [3000, 900, 10]
+    kp, vp, table = make_cache(210, lens, nkv, d, page, BF, dev)
+    q = normal(211, sum(new), nq, d, device=dev)
+    hk, hv, ht = host(kp), host(vp), host(table)
+    for bad in (False, True):
+        t, status = table.clone(), ints([0], dev)
+        if bad:
+            t[0, 40], ht[0, 40] = 1 << 28, -1
+        out = K.paged_attention_prompt(q, kp, vp, t, ints(lens, dev), offsets(new, dev), status=status)
+        assert int(status.item()) == (3 if bad else 0)
+        want, bound = oracle_rows(q, lambda b: (opaged.gather(hk, ht[b], lens[b]), opaged.gather(hv, ht[b], lens[b])),
+                                  [0, 20, 21, 21], d ** -0.5, True, BF, UNIT[BF])
+        check(f"cut over pages, bad {bad}", out, want, bound)
+
+
 def test_packed_takes_slices_of_one_projection(cuda_device):
     dev, nq, nkv, d, new = cuda_device, 8, 2, 128, [70, 9, 200]
     qkv = normal(71, sum(new), nq + 2 * nkv, d, device=dev)
@@ -291,6 +351,41 @@ def test_what_a_row_may_not_see_does_not_reach_it(cuda_device, bad):
             if vv is vb:  # and the rows that see the value have it
                 assert not torch.isfinite(got[at:last]).all(-1).any()
             assert first <= at
+
+
+def test_what_a_row_may_not_see_does_not_reach_it_in_cut_items(cuda_device):
+    dev, nq, nkv, d, n, m = cuda_device, 4, 1, 128, 40, 3000
+    q = normal(220, n, nq, d, device=dev)
+    k, v = normal(221, m, nkv, d, device=dev), normal(222, m, nkv, d, device=dev)
+    clean = K.packed_attention(q, k, v, offsets([n], dev), offsets([m], dev))
+    for at in (m - 1, m - 20, 100):
+        vb = v.clone()
+        vb[at] = float("nan")
+        got = K.packed_attention(q, k, vb, offsets([n], dev), offsets([m], dev))
+        sees = torch.arange(n, device=dev) + m - n >= at
+        assert torch.isnan(got[sees]).all() and torch.isfinite(got[~sees]).all()
+        err = (got[~sees].double() - clean[~sees].double()).abs()
+        assert bool((err <= 4 * UNIT[BF] * clean[~sees].double().abs() + 4 * UNIT[BF]).all())
+
+
+def test_scores_that_are_not_finite_reach_the_rows_that_see_them(cuda_device):
+    dev, d = cuda_device, 128
+    for dtype in (BF, HF):
+        q = normal(230, 200, 2, d, dtype=dtype, device=dev)
+        k, v = normal(231, 200, 2, d, dtype=dtype, device=dev), normal(232, 200, 2, d, dtype=dtype, device=dev)
+        k[150, 1] = float("nan")
+        q[20, 0] = float("nan")
+        got = K.packed_attention(q, k, v, offsets([200], dev))
+        bad = torch.zeros(200, 2, dtype=torch.bool, device=dev)
+        bad[150:, 1] = True
+        bad[20, 0] = True
+        assert torch.equal(torch.isnan(got).all(-1), bad) and torch.equal(torch.isnan(got).any(-1), bad)
+        out = K.paged_attention_decode(q[19:21], k[:, None].transpose(0, 1).reshape(1, 200, 2, d)[:, :192].transpose(1, 2)
+                                       .reshape(1, 2, 6, 32, d).transpose(1, 2)[0].contiguous(),
+                                       v[:192].transpose(0, 1).reshape(2, 6, 32, d).transpose(0, 1).contiguous(),
+                                       ints([list(range(6))] * 2, dev), ints([192, 192], dev))
+        want = torch.tensor([[False, True], [True, True]], device=dev)
+        assert torch.equal(torch.isnan(out).all(-1), want) and torch.equal(torch.isnan(out).any(-1), want)
 
 
 @pytest.mark.parametrize("dtype,nq,nkv,d,page", [(BF, 8, 2, 128, 16), (BF, 4, 1, 128, 64), (HF, 6, 2, 64, 32),
