@@ -407,6 +407,24 @@ def test_prompt_over_pages(cuda_device, dtype, nq, nkv, d, page, order):
 
 
 # ------------------------------------------------------------------------------------ together
+def test_a_single_token_is_as_exact_by_either_entry_point(cuda_device):
+    """One new token through the prompt entry points is held to the decode kernel's bound."""
+    dev = cuda_device
+    for dtype, nq, nkv, d, lens in ((BF, 8, 2, 128, [1000, 3, 129]), (HF, 7, 1, 64, [2000]), (HF, 4, 1, 128, [64, 65]),
+                                    (BF, 3, 3, 64, [500] * 8)):
+        kp, vp, table = make_cache(250, lens, nkv, d, 64, dtype, dev)
+        q = normal(251, len(lens), nq, d, dtype=dtype, device=dev)
+        ln, cu = ints(lens, dev), offsets([1] * len(lens), dev)
+        hk, hv, ht = host(kp), host(vp), host(table)
+        want, bound = oracle_rows(q, lambda b: (opaged.gather(hk, ht[b], lens[b]), opaged.gather(hv, ht[b], lens[b])),
+                                  list(range(len(lens) + 1)), d ** -0.5, True, dtype, DECODE_WEIGHT)
+        check("decode", K.paged_attention_decode(q, kp, vp, table, ln), want, bound)
+        check("prompt", K.paged_attention_prompt(q, kp, vp, table, ln, cu), want, bound)
+        packed = [torch.cat([torch.from_numpy(opaged.gather(x, ht[b], lens[b])) for b in range(len(lens))]).to(dtype).to(dev)
+                  for x in (hk, hv)]
+        check("packed", K.packed_attention(q, *packed, cu, offsets(lens, dev)), want, bound)
+
+
 def test_prompts_then_steps_through_one_cache(cuda_device):
     """Prompts in two chunks, then decode steps, through the pages: each attention result against the
     whole sequence in float64, from the rotated rows that the writes stored."""
