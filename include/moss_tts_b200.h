@@ -355,8 +355,8 @@ int mt_prefill_attention(const void* q, const void* k_cache, const void* v_cache
                          int nq, int nkv, int max_len, int flags, void* stream);
 
 /*
- * A paged key-value cache of one layer, for the four calls below (no counterpart in the reference,
- * whose cache is one contiguous buffer for one sequence, src/moss_tts/_runtime/llm.py:166-172).
+ * A paged key-value cache of one layer, for the calls below (no counterpart in the reference, whose
+ * static cache is one contiguous buffer for one sequence).
  * Key j of sequence b lies in row j % page_size of page page_table[b][j / page_size]:
  *   k_pages[page][head][row][head_dim], likewise v_pages; the strides of a page, a head and a row
  *   are in elements, multiples of 8; the head_dim elements of a row are adjacent.
@@ -397,7 +397,8 @@ int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_norm, co
  * Attention of one new token per sequence over its pages: out [batch][nq][D] =
  * softmax(scale q k^T) v over keys 0 .. kv_lens[b] - 1; q [batch] rows q_row elements apart, heads
  * q_head apart; query head h reads key head h / (nq / heads), nq / heads <= 64. A sequence of length 0
- * gives zeros. `workspace`: mt_paged_attention_decode_workspace bytes, 16-byte aligned, of any content; two
+ * gives zeros. Softmax weights are kept to two 16-bit numbers, sums to fp32. `workspace`:
+ * mt_paged_attention_decode_workspace bytes, 16-byte aligned, of any content; two
  * calls that may run at once have one each.
  */
 int mt_paged_attention_decode_workspace(long long* bytes);
@@ -407,11 +408,13 @@ int mt_paged_attention_decode(const void* q, int q_row, int q_head, const mt_pag
 /*
  * Attention of packed prompts: q [tokens_q], k and v [tokens_k] rows with their row and head strides
  * in elements; sequence b holds query rows cu_q[b] .. cu_q[b + 1] - 1 and key rows cu_k[b] ..
- * cu_k[b + 1] - 1 (int32 [batch + 1]). The last query stands at the last key: with causal != 0, query
+ * cu_k[b + 1] - 1 (int32 [batch + 1]); query heads 1 to 64 a key head. The last query stands at the last key: with causal != 0, query
  * i of n sees keys 0 .. len - n + i, which for len < n leaves the first rows without a key (zeros).
- * out [tokens_q][nq][D]; rows outside every sequence are left as they were. `workspace`:
+ * out [tokens_q][nq][D], 32-byte aligned; rows outside every sequence are left as they were. Softmax weights
+ * round to the type (calls of more than 512 rows tokens_q * nq); sums and statistics are fp32. A value or key
+ * that is not finite reaches the rows that may see it and no other. `workspace`:
  * mt_prompt_attention_workspace bytes (0 where the call's sizes need none; `keys` = tokens_k, or max_pages *
- * page_size), 16-byte aligned, of any content, one for each call that may run at once; NULL does without, to
+ * page_size), 32-byte aligned, of any content, one for each call that may run at once; NULL does without, to
  * the cost of calls with few rows and many keys.
  */
 int mt_prompt_attention_workspace(int tokens, int batch, int keys, int nq, int nkv, int head_dim, long long* bytes);

@@ -23,8 +23,9 @@ struct WriteArgs {
 };
 
 constexpr int kThreads = 128;
-// Heads that a thread has on their way at once, and threads. Measured in a graph, 3357 rows of 48 heads and 4
-// rows: 128 threads with 6 heads 18.4 and 3.4 us, with 3 18.8 and 2.7, with 2 20.9 and 2.6.
+// Heads that a thread has on their way at once. Measured in a graph, 3357 rows of 48 heads and 4 rows: with 6
+// 18.4 and 3.4 us, with 3 18.8 and 2.7, with 2 20.9 and 2.6 (64 threads: the same). What bounds the many rows
+// is the chain of look-ups and the instructions of a head (issue slots 68% full), at 4.4 TB/s.
 constexpr int kAhead = 3;
 
 // Bound by HBM. A CTA has one token's kAhead x kGroups heads: D/8 lanes hold one head (16 bytes each), so the mean of squares is
