@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
     while (true) {
       r.len = clamped_len(p, b, nullptr);
       r.chunks = chunks_of(r.len);
-      if (w0 < before + (long)r.chunks * per_seq) break;
+      if (w0 < before + (long)r.chunks * per_seq || b + 1 >= p.batch) break;
       before += (long)r.chunks * per_seq;
       ++b;
     }
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
   __syncthreads();  // `merge` takes the slabs' place
   auto advance = [&]() {  // the next item, from its first chunk; false past the run's end
     at += r.c1 - r.c0;
-    if (at >= w1) return false;
+    if (at >= w1 || (r.b + 1 >= p.batch && r.kh + 1 >= p.heads && r.group + 1 >= a.groups)) return false;
     if (++r.group == a.groups) {
       r.group = 0;
       if (++r.kh == p.heads) {

@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto total = [&]() { return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y); };
 
-        if (__any_sync(0xffffffffu, last > Reference<T>::most)) move(last > Reference<T>::most, m + __log2f(last));
+        const bool far = live && last > Reference<T>::most;  // rows without a token hold anything
+        if (__any_sync(0xffffffffu, far)) move(far, m + __log2f(last));
         load(0);
         arrived(0);
         if (j == it.j0) {
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (FINE) {
           if constexpr (Reference<T>::kChecked) {  // fp16: the maximum first, as there is time for it
             const float to = maximum();
-            if (__any_sync(0xffffffffu, to - m > kSlack)) move(to - m > kSlack, to);
+            if (__any_sync(0xffffffffu, live && to - m > kSlack)) move(to - m > kSlack, to);
             load(0);
             arrived(0);
           }
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               weights(c, ref, pw + 16 * c, nullptr);
               if (c + 1 < NC) arrived(c + 1);
             }
-            if (taken_again || !__any_sync(0xffffffffu, total() > Reference<T>::fits)) break;
+            if (taken_again || !__any_sync(0xffffffffu, live && total() > Reference<T>::fits)) break;
             const float to = maximum();
             move(to > m, to);
             sum[0] = sum[1] = make_float2(0.f, 0.f);
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait_for(&o_full[i], items++ & 1, dead);
       fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float odd = 0.f;  // not zero once an element is infinite or NaN
+      float odd = l * 0.f;  // not zero once an element, or the sum, is infinite or NaN
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t ow[32];
@@ -763,8 +764,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (SPLIT) {
         if (n) wait_for(&item_empty, (n - 1) & 1, dead);
         const int piece = blockIdx.x - w * cut, tiles = it.j1;
-        it.j0 = (int)((unsigned)(tiles * piece) / (unsigned)cut);  // at most 2^23 tiles x 148 pieces
-        it.j1 = (int)((unsigned)(tiles * (piece + 1)) / (unsigned)cut);
+        it.j0 = (int)((unsigned)tiles * piece / (unsigned)cut);  // at most 2^24 tiles x 148 pieces
+        it.j1 = (int)((unsigned)tiles * (piece + 1) / (unsigned)cut);
       }
       if (lane == 0) {
         item_s = it;
@@ -852,7 +853,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) prompt_join(const __grid_const
     m = top;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  float odd = 0.f;
+  float odd = l * 0.f;
   uint32_t w[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {

@@ -286,6 +286,23 @@ def test_packed_first_key_far_from_the_others(cuda_device, dtype, first):
     check(f"first key {first} {dtype}", got, want, bound)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rise", [30.0, 80.0, 87.3, 88.0, 95.0])
+@pytest.mark.parametrize("keys", [100, 300, 3000])
+def test_packed_weights_near_the_end_of_their_range(cuda_device, dtype, rise, keys):
+    """The first key's score is 0, the others lie `rise` above it: beside it their weights add up to up to
+    fp32's largest number and beyond, with values so small that their products do not."""
+    dev, d, n = cuda_device, 64, 40
+    q = torch.zeros(n, 16, d, device=dev, dtype=dtype)
+    q[..., 0] = 1
+    k = torch.zeros(keys, 1, d, device=dev, dtype=dtype)
+    k[1:, 0, 0] = 1
+    v = normal(83, keys, 1, d, dtype=torch.float32).mul(0.01).to(dtype).to(dev)
+    got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), scale=rise)
+    want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], rise, True, dtype, UNIT[dtype])
+    check(f"rise of {rise} over {keys} keys {dtype}", got, want, bound)
+
+
 def test_packed_many_short_sequences(cuda_device):
     """More items than CTAs, taken on demand, among them empty sequences."""
     r = np.random.default_rng(78)
