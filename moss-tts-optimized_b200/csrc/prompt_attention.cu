@@ -549,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait_for(&o_full[i], items++ & 1, dead);
       fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float odd = l * 0.f;  // not zero once an element, or the sum, is infinite or NaN
+      // not zero once an element, or the sum, is infinite or NaN; four chains
+      float2 odd2[2] = {make_float2(l * 0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t ow[32];
@@ -562,9 +563,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-              const float f0 = __uint_as_float(ow[16 * e + 2 * x]) * inv, f1 = __uint_as_float(ow[16 * e + 2 * x + 1]) * inv;
-              odd = fmaf(f0, 0.f, fmaf(f1, 0.f, odd));
-              w[x] = Elem<T>::pack(f0, f1);
+              const float2 zero = make_float2(0.f, 0.f);
+              const float2 f = fma2(make_float2(__uint_as_float(ow[16 * e + 2 * x]), __uint_as_float(ow[16 * e + 2 * x + 1])),
+                                    make_float2(inv, inv), zero);
+              odd2[x & 1] = fma2(f, zero, odd2[x & 1]);
+              w[x] = Elem<T>::pack(f.x, f.y);
             }
             store32(dst + 64 * c + 32 * e, w);
           }
@@ -573,6 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[i]);
+      const float odd = (odd2[0].x + odd2[0].y) + (odd2[1].x + odd2[1].y);
       unsigned again = __ballot_sync(0xffffffffu, live && !(odd == 0.f));
       while (again) {
         const int src = __ffs(again) - 1;
