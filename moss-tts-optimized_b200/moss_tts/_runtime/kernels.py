@@ -185,14 +185,17 @@ def _strides3(name, t, heads, d):
     return row, head
 
 
+def _no_backward(a, b, c=None):
+    if (a.requires_grad or b.requires_grad or c is not None and c.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("There is no backward pass: inputs that require a gradient need torch.no_grad()")
+
+
 def _query(q, nkv, d):
     """(tokens, heads, row stride, head stride, device index) of the queries."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         raise ValueError("CUDA tensors required (there is no CPU path)")
     if q.dtype not in _TYPES:
         raise ValueError("bf16 or fp16 tensors required")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise ValueError("This attention has no backward pass")
     if q.ndim != 3:
         raise ValueError("q must be [rows, heads, D]")
     tokens, nq, dq = q.shape
@@ -225,6 +228,12 @@ def _out(out, shape, like):
             or not out.is_contiguous() or out.data_ptr() & 31:
         raise ValueError(f"out must be a contiguous, 32-byte aligned {like.dtype} tensor {tuple(shape)} on the "
                          "queries' device")
+    # rows are read by other blocks than the one that writes them, and some a second time
+    if out.numel() and like.numel():
+        at, first = out.data_ptr(), like.data_ptr()
+        if at < first + 2 * (1 + sum((n - 1) * x for n, x in zip(like.shape, like.stride()))) \
+                and first < at + 2 * out.numel():
+            raise ValueError("out must not lie in the queries' memory")
     return out
 
 
@@ -289,7 +298,8 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     ``[pages, nkv, page_size, D]`` (any strides with adjacent D; page_size a power of two, 16 to 256; D 64 or
     128). ``kv_lens`` int32 ``[batch]`` counts each sequence's tokens with the new ones; ``cu_seqlens`` int32
     ``[batch + 1]`` are the new tokens' offsets in ``qkv``, or None for one token per sequence. Returns the
-    rotated queries ``[tokens, nq, D]`` (in ``out`` if given); rows behind the last sequence are not written.
+    rotated queries ``[tokens, nq, D]`` (in ``out`` if given, which has memory of its own); rows behind the last
+    sequence are not written.
 
     Unlike ``qk_rope_decode``, whose intermediate roundings are the reference's, this rounds once, at the
     store. A page that is written must belong to one sequence. ``status`` (int32, one element) takes 1 for a
@@ -300,14 +310,14 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     dtype, dev = qkv.dtype, qkv.get_device()
     if dtype not in _TYPES or qkv.ndim != 2:
         raise ValueError("qkv must be bf16 or fp16 [tokens, (nq + 2 nkv) * D]")
-    if qkv.requires_grad and torch.is_grad_enabled():
-        raise ValueError("This operator has no backward pass")
+    _no_backward(qkv, q_weight, k_weight)
     tokens, width = qkv.shape
     row, one = qkv.stride()
     if tokens <= 1:
         row = width
     if one != 1 or row & 7 or row < width or row >= 1 << 31 or qkv.data_ptr() & 15:
         raise ValueError("qkv must have adjacent elements in 16-byte aligned rows")
+    _no_backward(k_pages, v_pages)
     kv, batch, _ = _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev)
     nkv, d = k_pages.shape[1], k_pages.shape[3]
     nq = width // d - 2 * nkv
@@ -340,12 +350,14 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
 
     ``q`` ``[batch, nq, D]`` (bf16 or fp16; rows and heads may be strided); query head h reads key head
     ``h // (nq / nkv)``. Returns ``softmax(scale q k^T) v`` over keys ``0 .. kv_lens[b] - 1``, ``[batch, nq, D]``
-    (in ``out`` if given); ``scale`` defaults to ``1 / sqrt(D)``. A sequence of length 0 gives zeros.
+    (in ``out`` if given, which has memory of its own); ``scale`` defaults to ``1 / sqrt(D)``. A sequence of
+    length 0 gives zeros.
     ``status`` as in ``qk_rope_paged``: a length beyond the page table (1) is cut, a page id outside the
     cache (3) reads as zeros.
     """
     _, nkv, _, d = k_pages.shape
     rows, nq, row, head, dev = _query(q, nkv, d)
+    _no_backward(q, k_pages, v_pages)
     kv, batch, _ = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
     if rows != batch:
         raise ValueError("page_table must have a row for each query row")
@@ -363,13 +375,15 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, s
     may be strided, so slices of one ``q | k | v`` projection do); ``cu_seqlens_q`` / ``cu_seqlens_k`` int32
     ``[batch + 1]`` row offsets, the second None where they are the same. The last query of a sequence stands
     at its last key: with ``causal``, query i of n sees keys ``0 .. len - n + i``; a query without a key gives
-    zeros. Returns ``[tokens, nq, D]`` (in ``out`` if given); rows outside every sequence are not written.
+    zeros. Returns ``[tokens, nq, D]`` (in ``out`` if given, which has memory of its own); rows outside every
+    sequence are not written.
     """
     shape = k.shape
     if len(shape) != 3 or v.shape != shape:
         raise ValueError("k and v must be [tokens, nkv, D]")
     tokens_k, nkv, d = shape
     tokens, nq, row, head, dev = _query(q, nkv, d)
+    _no_backward(q, k, v)
     dtype = q.dtype
     if k.dtype is not dtype or v.dtype is not dtype or k.get_device() != dev or v.get_device() != dev:
         raise ValueError("k and v must have the queries' type and device")
@@ -404,6 +418,7 @@ def paged_attention_prompt(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens,
     """
     _, nkv, _, d = k_pages.shape
     tokens, nq, row, head, dev = _query(q, nkv, d)
+    _no_backward(q, k_pages, v_pages)
     kv, batch, most = _paged(k_pages, v_pages, page_table, kv_lens, q.dtype, dev)
     cu = _ints("cu_seqlens", cu_seqlens, batch + 1, dev)
     st = _status(status, dev)

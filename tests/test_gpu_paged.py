@@ -559,3 +559,39 @@ def test_refusals_on_the_device(cuda_device):
         a = {"k": k, "v": k, "cu": ints([0, 1], dev)} | bad
         with pytest.raises(ValueError):
             K.packed_attention(q, a["k"], a["v"], a["cu"], ints([0, 5], dev))
+
+
+def test_inputs_that_require_a_gradient_are_refused(cuda_device):
+    dev = cuda_device
+    kp, vp, table = make_cache(154, [20], 2, 64, 16, BF, dev)
+    q, ln, cu = normal(155, 1, 4, 64, device=dev), ints([20], dev), ints([0, 1], dev)
+    k = normal(156, 5, 2, 64, device=dev)
+    qkv, w = normal(157, 1, 8 * 64, device=dev), normal(158, 64, device=dev)
+    cos, sin = (t.to(BF).to(dev) for t in rope_tables(32, 64))
+    calls = [(K.paged_attention_decode, [q, kp, vp, table, ln]), (K.paged_attention_prompt, [q, kp, vp, table, ln, cu]),
+             (K.packed_attention, [q, k, k, cu, ints([0, 5], dev)]),
+             (K.qk_rope_paged, [qkv, w, w, cos, sin, kp, vp, table, ln, None, EPS])]
+    for call, args in calls:
+        for i, x in enumerate(args):
+            if not isinstance(x, torch.Tensor) or x.dtype != BF or x is cos or x is sin:
+                continue
+            with_grad = args[:i] + [x.detach().clone().requires_grad_()] + args[i + 1:]
+            with pytest.raises(ValueError, match="no backward pass"):
+                call(*with_grad)
+            with torch.no_grad():
+                call(*with_grad)
+
+
+def test_out_in_the_queries_memory_is_refused(cuda_device):
+    dev = cuda_device
+    kp, vp, table = make_cache(159, [20, 3], 2, 64, 16, BF, dev)
+    memory = normal(160, 5, 4, 64, device=dev)
+    q, ln, cu = memory[1:3], ints([20, 3], dev), ints([0, 1, 2], dev)
+    k = normal(161, 5, 2, 64, device=dev)
+    for out in (q, memory[:2], memory[2:4]):
+        for call in (lambda o: K.paged_attention_decode(q, kp, vp, table, ln, out=o),
+                     lambda o: K.paged_attention_prompt(q, kp, vp, table, ln, cu, out=o),
+                     lambda o: K.packed_attention(q, k, k, cu, ints([0, 3, 5], dev), out=o)):
+            with pytest.raises(ValueError, match="memory"):
+                call(out)
+            call(memory[3:])
