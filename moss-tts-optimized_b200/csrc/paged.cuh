@@ -103,7 +103,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int batch, int t, int 
 
 // softmax(scale q k^T) v of one query row over keys 0..n-1 by one warp, lane l holding elements
 // [l D/32, (l + 1) D/32) of q (scaled by scale * log2 e), k, v and the result. Keys past n are not
-// read. `rows(j, k, v)` gives key j's rows, null for a page that is not there (zeros).
+// read, nor keys behind one that leaves nothing but NaN. `rows(j, k, v)` gives key j's rows, null for a page
+// that is not there (zeros).
 template <typename T, int D, typename Rows>
 __device__ __forceinline__ void row_attention(const float (&q)[D / 32], int n, int lane, Rows rows,
                                               float (&o)[D / 32]) {
@@ -153,6 +154,10 @@ __device__ __forceinline__ void row_attention(const float (&q)[D / 32], int n, i
         o[2 * e + 1] = fmaf(p, vf.y, o[2 * e + 1]);
       }
     }
+    bool settled = true;  // once all is NaN it stays so
+#pragma unroll
+    for (int e = 0; e < E; ++e) settled = settled && o[e] != o[e];
+    if (__all_sync(0xffffffffu, settled || l != l)) break;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll

@@ -21,7 +21,7 @@
 // special-function unit, one exponential a score; it takes 3270, for each tile goes round a chain that
 // nothing shortens: scores seen 300 cycles after their product, weights 1840, seen by the issuing lane 250
 // to 400, products 790. Measured, bf16, 32 query and 8 key heads of 128, in a graph: 8191 causal tokens
-// 432 us (1.27 PFLOP/s; 507 us under the power cap of minutes of it), 16 prompts of 1 to 1024 tokens 87 us,
+// 432 us (1.27 PFLOP/s; 507 us under the power cap of minutes of it), 16 prompts of 1 to 1024 tokens 86 us,
 // 48 tokens behind 16001 keys 34 us. Tried and slower: two issuing warps (545 us: the tiles fall into step
 // and meet at either unit), sixteen softmax warps with two threads a row (441), a part of the exponentials
 // by polynomial (470: packed fp32 instructions take two issue slots), the output turned through shared
@@ -51,7 +51,7 @@ constexpr int kTile = 128;      // query rows of a tile and keys of a step
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kZeroWarp = 10, kFeedWarp = 11, kThreads = 384;
 constexpr int kWalkers = 11;    // warps that take an item from the feed
 constexpr int kTmemCols = 512;
-// A row that needs the slow path (below) keeps its warp busy for long; far above that all the same.
+// Far above a step's microseconds; the time that a warp spends on the slow path (row_again) does not count.
 constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
 // Softmax weights round to the values' type for the tensor core, by 2^-9 of themselves on average for bf16:
 // with the rounding of the output that makes an error sqrt(2) times the output's alone. Calls of up to
@@ -201,15 +201,20 @@ __device__ int pieces(const PromptArgs& a, const Pages& p, int lane) {
 
 // Waits for a phase. Where that does not come, the kernel gives up: `dead` ends this and every later
 // wait at once, and the warps run through what is left of their work, to no use but within bounds.
+// dead[1] counts the warps on the slow path: half a second for 32 rows of 65536 keys, and it ends by itself.
+// The clock is read in a function of its own: the waits of 20 places stay short (16 prompts 87.9 us with it
+// in line, 85.9 without).
+__device__ __noinline__ unsigned long long waited_long(unsigned long long since, volatile int* dead) {
+  const unsigned long long now = globaltimer_ns();
+  if (since == 0 || dead[1]) return now;
+  if (now - since > kDeadlineNs) *dead = 1;
+  return since;
+}
 __device__ __forceinline__ void wait_for(uint64_t* bar, unsigned parity, volatile int* dead) {
-  unsigned long long t0 = 0;
+  unsigned long long since = 0;
   for (unsigned tries = 0; !mbar_try_wait(bar, parity); ++tries) {
-    if (tries % 64 == 63 || *dead) {
-      if (*dead) return;
-      const unsigned long long now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > kDeadlineNs) *dead = 1;
-    }
+    if (*dead) return;
+    if (tries % 64 == 63) since = waited_long(since, dead);
   }
 }
 // For copies and matrix products in flight when the kernel gives up: bounded, whatever `dead` says.
@@ -248,6 +253,20 @@ __device__ __noinline__ void row_again(const PromptArgs* args, const Pages* page
   for (int e = 0; e < E / 2; ++e) op[e] = Elem<T>::pack(o[2 * e], o[2 * e + 1]);
 }
 
+// The warp's rows of a mask, a lane a row; `busy` counts the warps at it.
+template <typename T, int D, bool PAGED>
+__device__ __noinline__ void rows_again(const PromptArgs* args, const Pages* pages, int b, int kh, int k0, unsigned again,
+                                        int seen, int row, int h, int* busy) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) atomicAdd(busy, 1);
+  for (; again; again &= again - 1) {
+    const int src = __ffs(again) - 1;
+    row_again<T, D, PAGED>(args, pages, b, kh, k0, __shfl_sync(0xffffffffu, seen, src), __shfl_sync(0xffffffffu, row, src),
+                           __shfl_sync(0xffffffffu, h, src));
+  }
+  if (lane == 0) atomicSub(busy, 1);
+}
+
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;                  // a tile is `halves` boxes of 64 elements a row
@@ -270,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Item item_s;
   __shared__ __align__(8) uint64_t answered, item_full, item_empty;
   __shared__ uint32_t tmem_s;
-  __shared__ int dead_s;
-  volatile int* dead = &dead_s;
+  __shared__ int dead_s[2];
+  volatile int* dead = dead_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;  // Q_0, Q_1, then the ring
   const uint32_t ring = smem + 2 * L::kTileBytes;
@@ -301,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&item_full, 1);
       mbar_init(&item_empty, kWalkers);
       mbar_init(&drained, 1);
-      dead_s = 0;
+      dead_s[0] = dead_s[1] = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
@@ -577,13 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[i]);
       const float odd = (odd2[0].x + odd2[0].y) + (odd2[1].x + odd2[1].y);
-      unsigned again = __ballot_sync(0xffffffffu, live && !(odd == 0.f));
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        row_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, __shfl_sync(0xffffffffu, seen, src),
-                               it.q0 + __shfl_sync(0xffffffffu, t, src), __shfl_sync(0xffffffffu, h, src));
-      }
+      const unsigned again = __ballot_sync(0xffffffffu, live && !(odd == 0.f));
+      if (again) rows_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, again, seen, it.q0 + t, h, &dead_s[1]);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ tensor core
@@ -794,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-    if (dead_s && lane == 0) atomicExch(&g_prompt_error, 1);
+    if (dead_s[0] && lane == 0) atomicExch(&g_prompt_error, 1);
   }
 }
 

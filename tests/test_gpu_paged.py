@@ -8,7 +8,7 @@ import torch
 from oracle import paged as opaged
 from paged_cases import UNIT, check, host, ints, make_cache, normal, offsets, oracle_rows
 
-from moss_tts._runtime import kernels as K
+from moss_tts._runtime import kernels as K, native
 from moss_tts._runtime.engine import rope_tables
 
 pytestmark = pytest.mark.gpu
@@ -595,3 +595,34 @@ def test_out_in_the_queries_memory_is_refused(cuda_device):
             with pytest.raises(ValueError, match="memory"):
                 call(out)
             call(memory[3:])
+
+
+def test_rows_with_a_value_that_is_not_finite_in_a_very_long_cache(cuda_device):
+    """640,000 keys: rows that are computed again, one by one, take seconds, which is no expired wait. All pages
+    hold the same rows (the first with one element that is not finite), so that key j of a page counts as often
+    as a row sees it."""
+    dev, nq, nkv, d, page, n, long = cuda_device, 4, 1, 128, 64, 64, 10000
+    kp, vp = normal(162, 2, nkv, page, d, device=dev), normal(163, 2, nkv, page, d, device=dev)
+    kp[1], vp[1] = kp[0], vp[0]
+    vp[1, 0, 5, 3] = float("nan")
+    batch = 80  # enough items that none is cut
+    table = torch.zeros(batch, long, device=dev, dtype=torch.int32)
+    table[0, 0] = 1
+    lens, new = [long * page] + [page] * (batch - 1), [n] + [1] * (batch - 1)
+    q = normal(164, sum(new), nq, d, device=dev)
+    native.error_word(clear=True)
+    got = K.paged_attention_prompt(q, kp, vp, table, ints(lens, dev), offsets(new, dev))
+    assert native.error_word() == 0
+    assert torch.isnan(got[:n, :, 3]).all()
+    got[:n, :, 3] = 0
+    hk, hv = (host(x[0]).transpose(1, 0, 2) for x in (kp, vp))
+    want, bound = oracle_rows(q, lambda b: (hk, hv), [0] + list(range(n, n + batch)), d ** -0.5, False, BF, UNIT[BF])
+    for t in range(n):
+        seen = long * page - n + t + 1
+        p = np.exp(d ** -0.5 * host(q)[t] @ hk[:, 0].T) * (seen // page + (np.arange(page) < seen % page))
+        p /= p.sum(-1, keepdims=True)
+        want[t] = p @ hv[:, 0]
+        # a rounding of the weights' sum and one of an element's for every key that is added
+        bound[t] = UNIT[BF] * np.abs(want[t]) + 2 * 2.0 ** -24 * seen * (p @ np.abs(hv[:, 0]))
+    want[:n, :, 3] = 0
+    check("very long", got, want, bound)
