@@ -626,3 +626,19 @@ def test_rows_with_a_value_that_is_not_finite_in_a_very_long_cache(cuda_device):
         bound[t] = UNIT[BF] * np.abs(want[t]) + 2 * 2.0 ** -24 * seen * (p @ np.abs(hv[:, 0]))
     want[:n, :, 3] = 0
     check("very long", got, want, bound)
+
+
+@pytest.mark.parametrize("tokens_each,nq", [(700, 4), (9, 2)])
+def test_empty_sequences_between_others_change_nothing(cuda_device, tokens_each, nq):
+    """A padded batch: blocks without an item outnumber the others, and are taken by those."""
+    dev, d = cuda_device, 64
+    real = [tokens_each - 3 * i for i in range(3)]
+    new = [0] * 5 + [real[0]] + [0] * 1200 + [real[1], real[2]] + [0] * 3000
+    q, k, v = (normal(170 + i, sum(real) + 11, nq, d, device=dev) for i in range(3))
+    out = torch.full_like(q, 7.0)
+    K.packed_attention(q, k, v, offsets(new, dev), out=out)
+    assert bool((out[sum(real):] == 7.0).all())  # rows behind the last sequence
+    cu = [0] + list(np.cumsum(real))
+    hk, hv = host(k), host(v)
+    want, bound = oracle_rows(q[:cu[-1]], lambda b: (hk[cu[b]:cu[b + 1]], hv[cu[b]:cu[b + 1]]), cu, d ** -0.5, True, BF, UNIT[BF])
+    check("padded batch", out[:cu[-1]], want, bound)
