@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
     const int per_chunk = kChunk / rows;                  // boxes of a chunk, for either half of K and of V
     const int box = lane / (2 * R::kHalves), what = lane - box * 2 * R::kHalves;  // page, then half, K or V
     do {
+      if (r.len == 0) continue;
       const int* table = p.table + r.b * p.table_row;
       int ids = 0, first = 1 << 30;  // a lane a box: the page ids of the 32 boxes from `first` on
       for (int c = r.c0; c < r.c1; ++c, ++idx) {
@@ -275,6 +276,12 @@ __global__ void __launch_bounds__(kDecodeThreads, kCtasPerSm)
   const int tok0 = 16 * warp;
   do {
     const int heads = min(kHeads, a.rep - r.group * kHeads), row0 = r.b * a.nq + r.kh * a.rep + r.group * kHeads;
+    if (r.len == 0) {  // one chunk of nothing, always whole: zeros
+      for (int x = tid; x < heads * D / 8; x += kConsumers * 32)
+        reinterpret_cast<uint4*>(a.out + (long long)row0 * D * 2)[x] = make_uint4(0, 0, 0, 0);
+      if (tid == 0 && at + 1 >= w1) a.joins[run] = make_int4(0, 0, 0, 0);
+      continue;
+    }
     uint32_t qa[NK][2];
     const char* qp = a.q + (r.b * a.q_row + (long long)(r.kh * a.rep + r.group * kHeads + g) * a.q_head) * 2;
 #pragma unroll
