@@ -398,7 +398,8 @@ int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_norm, co
  * Attention of one new token per sequence over its pages: out [batch][nq][D] =
  * softmax(scale q k^T) v over keys 0 .. kv_lens[b] - 1; q [batch] rows q_row elements apart, heads
  * q_head apart; query head h reads key head h / (nq / heads), nq / heads <= 64. A sequence of length 0
- * gives zeros. Softmax weights are kept to two 16-bit numbers, sums to fp32. `workspace`:
+ * gives zeros. Softmax weights are kept to two 16-bit numbers, sums to fp32; an infinite value that a row sees
+ * may leave NaN there. `workspace`:
  * mt_paged_attention_decode_workspace bytes, 16-byte aligned, of any content; two
  * calls that may run at once have one each.
  */

@@ -351,7 +351,7 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
     ``q`` ``[batch, nq, D]`` (bf16 or fp16; rows and heads may be strided); query head h reads key head
     ``h // (nq / nkv)``. Returns ``softmax(scale q k^T) v`` over keys ``0 .. kv_lens[b] - 1``, ``[batch, nq, D]``
     (in ``out`` if given, which has memory of its own); ``scale`` defaults to ``1 / sqrt(D)``. A sequence of
-    length 0 gives zeros.
+    length 0 gives zeros; an infinite value may leave NaN.
     ``status`` as in ``qk_rope_paged``: a length beyond the page table (1) is cut, a page id outside the
     cache (3) reads as zeros.
     """
