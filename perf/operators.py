@@ -11,7 +11,6 @@ it is false; ``exact`` is the definition in 64 bits, sequence by sequence.
 A case's lengths follow from its own ``ragged`` number: ``batch`` sequences with ``new_low``..``new`` new
 tokens behind ``past_low``..``past`` tokens that the cache holds already.
 """
-import functools
 import math
 import random
 import sys
@@ -186,8 +185,7 @@ def _kernels(s):
     return k.packed_attention(s["q"], s["k"], s["v"], s["cu"], s["cu_k"], causal=s["case"]["causal"], out=s["out"])
 
 
-@functools.cache
-def _framework():  # imported once, as a program does
+def _framework():
     root = str(Path(__file__).resolve().parent.parent / "moss-tts-optimized_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
