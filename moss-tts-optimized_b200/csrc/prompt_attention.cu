@@ -774,7 +774,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       wait_for(&answered, asked++ & 1, dead);
-      return *dead ? -1 : taken_block(&answer);
+      const int block = *dead ? -1 : taken_block(&answer);
+      // this lane's read comes before the next answer, which the asynchronous proxy writes to the same place
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      return block;
     };
     for (unsigned n = 0;; ++n) {
       int w = blockIdx.x, cut = 1;
