@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, far)) move(far, m + __log2f(last));
         load(0);
         arrived(0);
-        if (j == it.j0) {
-          m = score(sw[0][0], 0) * k;
-        } else if (__any_sync(0xffffffffu, live && m == -INFINITY)) {  // no key seen yet, or infinitely low ones
+        if (j == it.j0) m = score(sw[0][0], 0) * k;
+        // no key seen yet, or infinitely low ones: no reference to weigh the others against, this step's neither
+        if (__any_sync(0xffffffffu, live && left > 0 && m == -INFINITY)) {
           const float to = maximum();
           move(m == -INFINITY && to > m, to);
           load(0);

@@ -31,3 +31,53 @@ def test_blocks_taken_one_after_the_other_without_an_item(cuda_device, slots):
     hk, hv = host(k), host(v)
     want, bound = oracle_rows(q, lambda b: (hk[at[b]:at[b + 1]], hv[at[b]:at[b + 1]]), at, d ** -0.5, True, BF, UNIT[BF])
     check("padded batch, repeated", first, want, bound)
+
+
+def _first_element(dev, dtype, n, heads, d):
+    q = torch.zeros(n, heads, d, device=dev, dtype=dtype)
+    q[..., 0] = 1
+    return q
+
+
+# ------------------------------------------------------------------------------------ infinitely low scores
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,heads,keys", [(48, 16, 60), (48, 16, 128), (48, 16, 300), (48, 16, 3000), (3, 4, 60), (3, 4, 300),
+                                          (3, 4, 3000)])
+@pytest.mark.parametrize("others", [0.0, -120.0, 60.0])
+def test_keys_of_infinitely_low_score_count_for_nothing(cuda_device, dtype, n, heads, keys, others):
+    """Keys with an element of -inf against a positive one of the queries have a weight of 0, wherever they
+    stand (the first key, the first of a tile, whole tiles); the others keep theirs, whose scores lie around
+    ``others``. The prompt forms and the decode give what float64 gives without those keys."""
+    dev, d = cuda_device, 128
+    q = normal(320, n, heads, d, dtype=dtype, device=dev)
+    q[..., 0] = 1
+    q[..., 1] = others * d ** 0.5 / 8
+    k, v = normal(321, keys, 1, d, dtype=dtype, device=dev), normal(322, keys, 1, d, dtype=dtype, device=dev)
+    k[:, 0, 1] = 8
+    for low in ([0], [0, 1, 2, keys - 1], list(range(0, keys, 128)), list(range(min(128, keys - 1))), list(range(0, keys, 2))):
+        kk = k.clone()
+        kk[low, 0, 0] = -float("inf")
+        rest = np.setdiff1d(np.arange(keys), low)
+        want, bound = oracle_rows(q, lambda b: (host(k)[rest], host(v)[rest]), [0, n], d ** -0.5, False, dtype, UNIT[dtype])
+        got = K.packed_attention(q, kk, v, offsets([n], dev), offsets([keys], dev), causal=False)
+        check(f"{len(low)} of {keys} keys infinitely low {dtype}", got, want, bound)
+        pages = -(-keys // 64)
+        pool = torch.zeros(2, pages * 64, 1, d, device=dev, dtype=dtype)
+        pool[0, :keys], pool[1, :keys] = kk, v
+        kp, vp = pool.view(2, pages, 64, 1, d).transpose(2, 3).contiguous()
+        table = torch.arange(pages, device=dev, dtype=torch.int32)[None].repeat(n, 1)
+        length = torch.full((n,), keys, device=dev, dtype=torch.int32)
+        check("decode", K.paged_attention_decode(q, kp, vp, table, length), want, bound)
+        got = K.paged_attention_prompt(q, kp, vp, table, length, offsets([1] * n, dev))
+        check("prompt over pages", got, want, bound)
+
+
+def test_rows_of_infinitely_low_scores_alone(cuda_device):
+    """Where every key's weight is 0 the row is zeros, by either entry point, also in cut items."""
+    dev, d = cuda_device, 128
+    for n, keys in ((40, 100), (40, 2000), (2, 2000)):
+        q = _first_element(dev, BF, n, 16, d)
+        k, v = torch.zeros(keys, 1, d, device=dev, dtype=BF), normal(330, keys, 1, d, device=dev)
+        k[..., 0] = -float("inf")
+        got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False)
+        assert bool((got == 0).all())
