@@ -67,7 +67,9 @@ constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
 //   the row is computed again (row_again).
 //   fp16 weights end at 2^16: a step whose weights add up to more than `fits` is taken again with its
 //   maximum, before the weights go out; they go out all at once.
-constexpr float kSlack = 8.f;
+// A move goes 2^kFarthest at the most, and the next step's the rest: ex2 makes a factor below 2^-126 zero, and a sum
+// of 2^127, which is finite, would be lost with the accumulator.
+constexpr float kSlack = 8.f, kFarthest = 120.f;
 constexpr int kFineRows = 512;
 template <typename T>
 struct Reference {
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto total = [&]() { return (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y); };
 
         const bool far = live && last > Reference<T>::most;  // rows without a token hold anything
-        if (__any_sync(0xffffffffu, far)) move(far, m + __log2f(last));
+        if (__any_sync(0xffffffffu, far)) move(far, m + fminf(__log2f(last), kFarthest));
         load(0);
         arrived(0);
         if (j == it.j0) m = score(sw[0][0], 0) * k;

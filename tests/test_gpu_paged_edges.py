@@ -81,3 +81,28 @@ def test_rows_of_infinitely_low_scores_alone(cuda_device):
         k[..., 0] = -float("inf")
         got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False)
         assert bool((got == 0).all())
+
+
+# ------------------------------------------------------------------------------------ scores far apart
+def _raised(dev, dtype, d, keys, raised):
+    """Keys whose first element is 0 but for ``raised`` {index: element}, values of 0.25 but 1.5 at those."""
+    k = torch.zeros(keys, 1, d, device=dev, dtype=dtype)
+    v = torch.full((keys, 1, d), 0.25, device=dev, dtype=dtype)
+    for at, x in raised.items():
+        k[at, 0, 0], v[at] = x, 1.5
+    return k, v
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,heads,d", [(40, 16, 64), (6, 4, 128), (24, 32, 128)])  # over 512 rows, and fewer
+@pytest.mark.parametrize("rise", [30.0, 60.0, 87.3, 87.4, 88.0, 88.7, 95.0, 300.0])
+def test_one_key_far_above_the_others(cuda_device, dtype, n, heads, d, rise):
+    """One weight of e^rise beside some of 1, in the first key tile, a later one, the last one; with the first
+    key, whose score the reference may start from, among the low ones."""
+    dev = cuda_device
+    q = _first_element(dev, dtype, n, heads, d)
+    for keys, at in ((200, 50), (200, 100), (300, 150), (300, 299), (1000, 70), (1000, 700), (3000, 2999), (100, 99)):
+        k, v = _raised(dev, dtype, d, keys, {at: 1.0})
+        got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False, scale=rise)
+        want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], rise, False, dtype, UNIT[dtype])
+        check(f"rise of {rise} at {at} of {keys} {dtype}", got, want, bound)
