@@ -538,12 +538,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int h = it.kh * a.rep + rhead;
       if constexpr (SPLIT) {
-        // a piece: the accumulator, the reference and the sum as they are
+        // A piece: the accumulator, the reference and the sum. The join weighs pieces by their references, so a
+        // power of two near the sum goes over to it: the largest weight may lie 2^127 above the reference.
+        const int up = min(max((__float_as_int(l) >> 23 & 255) - 127, 0), (int)kFarthest);
+        const float f = __int_as_float((127 - up) << 23);
         float* part = a.parts + (long long)blockIdx.x * (2 * kTile) * (D + 2);
         const int r = i * kTile + row;
         const bool none = n <= it.j0 || l == 0.f;  // nothing to add; -inf says so
-        part[2 * kTile * D + r] = none ? -INFINITY : m == -INFINITY ? 0.f : m;
-        part[2 * kTile * (D + 1) + r] = none ? 0.f : l;
+        part[2 * kTile * D + r] = none ? -INFINITY : (m == -INFINITY ? 0.f : m) + up;
+        part[2 * kTile * (D + 1) + r] = none ? 0.f : l * f;
         if (n <= it.j0) continue;
         wait_for(&o_full[i], items++ & 1, dead);
         fence_after();
@@ -553,6 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ld32(o_at + 32 * c, ow);
           wait_ld();
           hold<32>(ow);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
           if (live) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)

@@ -106,3 +106,22 @@ def test_one_key_far_above_the_others(cuda_device, dtype, n, heads, d, rise):
         got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False, scale=rise)
         want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], rise, False, dtype, UNIT[dtype])
         check(f"rise of {rise} at {at} of {keys} {dtype}", got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,heads", [(20, 4), (48, 16)])
+@pytest.mark.parametrize("rise", [30.0, 88.0, 88.7, 200.0])
+def test_raised_keys_of_cut_items_are_weighed_against_one_another(cuda_device, dtype, n, heads, rise):
+    """Pieces of an item start from references far apart, with their largest weights anywhere."""
+    dev, d, keys = cuda_device, 128, 3000
+    q = _first_element(dev, dtype, n, heads, d)
+    r = np.random.default_rng(310)
+    cases = [{0: 1.0, 2990: 0.9921875}, {2990: 0.9921875, 400: 1.0, 384: 1.0}, {768: 1.0, 100: 0.9921875}]
+    cases += [{int(at): float(x) for at, x in zip(r.integers(0, keys, 6), r.choice([1.0, 0.9921875, 0.984375, -1.0], 6))}
+              for _ in range(8)]
+    for raised in cases:
+        k, v = _raised(dev, dtype, d, keys, raised)
+        v += 0.125 * torch.arange(keys, device=dev)[:, None, None].remainder(7).to(dtype)
+        got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False, scale=rise)
+        want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], rise, False, dtype, UNIT[dtype])
+        check(f"pieces, rise of {rise} at {raised} {dtype}", got, want, bound)
