@@ -64,7 +64,7 @@ constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
 // moves when a step's weights add up to more than `most`, for the next step, which rescales the
 // accumulator (seldom: the largest of many scores is rarely far above the first). No maximum is looked for.
 //   bf16 weights have the range of fp32: scores that rise by 2^97 within one step leave an infinity, and
-//   the row is computed again (row_again).
+//   the item is taken once more, with the maximum of every step (kCareful).
 //   fp16 weights end at 2^16: a step whose weights add up to more than `fits` is taken again with its
 //   maximum, before the weights go out; they go out all at once.
 // A move goes 2^kFarthest at the most, and the next step's the rest: ex2 makes a factor below 2^-126 zero, and a sum
@@ -103,12 +103,16 @@ __device__ __forceinline__ void span_of(const int* cu, int b, int tokens, int& f
   n = max(min(cu[b + 1], tokens) - first, 0);
 }
 
+// What a warp is to do with what the feed lays out: an item; an item once more, now with the largest score of
+// every step; nothing, there is no further one.
+enum Mode { kItem, kCareful, kNone };
+
 struct __align__(16) Item {
   int b, kh, q0, lq, k0, len;  // sequence, key head, its rows
   int t0;                      // first token of query tile 0
   int seen[2];                 // keys that query tile i's last row sees
   int j0, j1;                  // key tiles of this piece of the item: [j0, j1), as far as a query tile reads
-  int none;                    // there is no further item
+  int mode;
 };
 // Key tiles of a query tile, and the keys that step j of them works on: 128, or 64 where the last
 // tile holds no more.
@@ -225,8 +229,8 @@ __device__ __forceinline__ void wait_for(uint64_t* bar, unsigned parity, volatil
 __device__ __forceinline__ void drain(uint64_t* bar, unsigned parity) { (void)pipe::mbar_wait_bounded(bar, parity); }
 
 // A tile multiplies masked weights (zeros) with values too: a value row that is not finite makes
-// rows that must not see it NaN. A row that comes out non-finite is computed again, by one warp, from
-// its own keys alone, so that it holds what its keys say.
+// rows that must not see it NaN. A row that comes out non-finite from its item's second pass too is computed
+// again, by one warp, from its own keys alone, so that it holds what its keys say.
 template <typename T, int D, bool PAGED>
 __device__ __noinline__ void row_again(const PromptArgs* args, const Pages* pages, int b, int kh, int k0, int seen,
                                        int row, int h) {
@@ -271,6 +275,49 @@ __device__ __noinline__ void rows_again(const PromptArgs* args, const Pages* pag
   if (lane == 0) atomicSub(busy, 1);
 }
 
+template <int N>
+__device__ __forceinline__ void scale_columns(uint32_t at, float f) {
+#pragma unroll
+  for (int c = 0; c < N; c += 32) {
+    uint32_t w[32];
+    ld32(at + c, w);
+    wait_ld();
+    hold<32>(w);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+    st32(at + c, w);
+  }
+}
+// What is needed seldom, as functions of their own: in line they cost the loops around them registers (16
+// prompts 88.6 us and 48 rows behind 16001 keys 36.6 with all three in line, 85.7 and 34.1 so). fp16, whose
+// reference moves sooner, scales in line (12 windows 57.2 us
+// otherwise, 56.1 so).
+template <int N>
+__device__ __noinline__ void scale_columns_seldom(uint32_t at, float f) {
+  scale_columns<N>(at, f);
+}
+// The largest of this lane's scores in `cols` columns, of which the first `left` count.
+__device__ __noinline__ float largest(uint32_t at, int cols, int left, float scale) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < cols; c += 32) {
+    uint32_t w[32];
+    ld32(at + c, w);
+    wait_ld();
+    hold<32>(w);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = fmaxf(top, c + e < left ? __uint_as_float(w[e]) * scale : -INFINITY);
+  }
+  return top;
+}
+
+// All warps of a CTA, at the end: whether the last item is to be taken again.
+__device__ __noinline__ bool goes_again(volatile int* dead, volatile int* flagged) {
+  __syncwarp();
+  pipe::named_sync(1, kThreads);
+  return !*dead && *flagged;
+}
+
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;                  // a tile is `halves` boxes of 64 elements a row
@@ -293,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Item item_s;
   __shared__ __align__(8) uint64_t answered, item_full, item_empty;
   __shared__ uint32_t tmem_s;
-  __shared__ int dead_s[2];
-  volatile int* dead = dead_s;
+  __shared__ int dead_s[2], flagged_s[2];
+  volatile int *dead = dead_s, *flagged = flagged_s;  // flagged: rows of item n & 1 came out infinite or NaN
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;  // Q_0, Q_1, then the ring
   const uint32_t ring = smem + 2 * L::kTileBytes;
@@ -324,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&item_full, 1);
       mbar_init(&item_empty, kWalkers);
       mbar_init(&drained, 1);
-      dead_s[0] = dead_s[1] = 0;
+      dead_s[0] = dead_s[1] = flagged_s[0] = flagged_s[1] = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
@@ -343,15 +390,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   Item it;
   unsigned taken = 0;  // items of this CTA so far
-  auto next = [&]() -> bool {  // the next item, as the feed warp has laid it out
-    wait_for(&item_full, taken++ & 1, dead);
-    const int4 *from = reinterpret_cast<const int4*>(&item_s);
-    int4 *to = reinterpret_cast<int4*>(&it);
+  // An item of which rows came out infinite or NaN is taken once more, with the largest score of every step as
+  // its reference (kCareful): finite scores, however far they rise, then cost no more than a second pass. All
+  // warps are done with item n - 2 when they have taken item n - 1, which the feed waits for before it lays out
+  // item n. Only for the last one all wait, once each, before they leave.
+  bool waited = false;
+  auto last_flagged = [&](unsigned n) {  // whether item n goes round again, behind which there is no other
+    waited = true;
+    return goes_again(dead, &flagged[n & 1]);
+  };
+  // The next item, as the feed warp has laid it out; `leaving` runs where there may be none.
+  auto next = [&](auto leaving) -> bool {
+    while (true) {
+      wait_for(&item_full, taken++ & 1, dead);
+      const int4 *from = reinterpret_cast<const int4*>(&item_s);
+      int4 *to = reinterpret_cast<int4*>(&it);
 #pragma unroll
-    for (int x = 0; x < 3; ++x) to[x] = from[x];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty);
-    return !*dead && !it.none;
+      for (int x = 0; x < 3; ++x) to[x] = from[x];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty);
+      if (!*dead && it.mode != kNone) return true;
+      leaving();
+      if (waited || !last_flagged(taken - 2)) return false;
+    }
   };
   if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ softmax, one thread a row
@@ -364,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // belongs to the largest score
     const bool plain = a.scale > 0.f;
     const float k = plain ? a.scale : 1.f;
-    while (next()) {
+    while (next([] {})) {
       const int t = it.t0 + i * a.tok + rtok;  // this row's token
       const bool live = rtok < a.tok && t < it.lq;
       const int n = min(tiles_of(it.seen[i]), it.j1), seen = live ? keys_seen(a, it, t) : 0;  // key tiles [j0, n)
@@ -383,36 +444,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (MASKED) s = c < left ? s : -INFINITY;
           return s;
         };
-        constexpr bool CHECKED = Reference<T>::kChecked && !FINE;
         auto move = [&](bool moves, float to) {  // of the rows that do, to another reference
           const float f = moves ? ex2(m - to) : 1.f;
           if (moves) m = to;
           l *= f;
           if (j == it.j0) return;
           // S of this step is there, so the product of the last one is done
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t ow[32];
-            ld32(o_at + 32 * c, ow);
-            wait_ld();
-            hold<32>(ow);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
-            st32(o_at + 32 * c, ow);
-          }
+          if constexpr (Reference<T>::kChecked)
+            scale_columns<D>(o_at, f);
+          else
+            scale_columns_seldom<D>(o_at, f);
         };
         auto maximum = [&]() {
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            uint32_t w[32];
-            ld32(s_at + 32 * c, w);
-            wait_ld();
-            hold<32>(w);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) top = max3(top, score(w[e], 32 * c + e), score(w[e + 1], 32 * c + e + 1));
-          }
-          return top * k;
+          return largest(s_at, COLS, MASKED ? left : kTile, plain ? 1.f : a.scale) * k;
         };
         const float2 k2 = make_float2(k, k);
         float2 sum[2];
@@ -453,9 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         arrived(0);
         if (j == it.j0) m = score(sw[0][0], 0) * k;
         // no key seen yet, or infinitely low ones: no reference to weigh the others against, this step's neither
-        if (__any_sync(0xffffffffu, live && left > 0 && m == -INFINITY)) {
+        const bool careful = it.mode == kCareful;
+        if (careful || __any_sync(0xffffffffu, live && left > 0 && m == -INFINITY)) {
           const float to = maximum();
-          move(m == -INFINITY && to > m, to);
+          move((careful || m == -INFINITY) && to > m, to);
           load(0);
           arrived(0);
         }
@@ -482,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           announce(&p_most[i]);
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[i]);
-        } else if constexpr (CHECKED) {
+        } else if constexpr (Reference<T>::kChecked) {
           uint32_t pw[COLS / 2];
 #pragma unroll 1
           for (int taken_again = 0;; taken_again = 1) {
@@ -550,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n <= it.j0) continue;
         wait_for(&o_full[i], items++ & 1, dead);
         fence_after();
+        float2 odd2 = make_float2(l * 0.f, 0.f);  // as below
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t ow[32];
@@ -557,13 +603,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_ld();
           hold<32>(ow);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * f);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 zero = make_float2(0.f, 0.f);
+            const float2 o = fma2(make_float2(__uint_as_float(ow[e]), __uint_as_float(ow[e + 1])), make_float2(f, f), zero);
+            odd2 = fma2(o, zero, odd2);
+            ow[e] = __float_as_uint(o.x), ow[e + 1] = __float_as_uint(o.y);
+          }
           if (live) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               store32(part + ((4 * c + e) * (2 * kTile) + r) * 8, reinterpret_cast<const uint32_t(&)[8]>(ow[8 * e]));
           }
         }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[i]);
+        // what is not finite even then is the join's to compute again
+        if (__any_sync(0xffffffffu, live && !none && !(odd2.x + odd2.y == 0.f)) && it.mode == kItem && lane == 0)
+          flagged[(taken - 1) & 1] = 1;
         continue;
       }
       char* dst = a.out + ((long long)(it.q0 + t) * a.nq + h) * D * 2;
@@ -606,7 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&o_free[i]);
       const float odd = (odd2[0].x + odd2[0].y) + (odd2[1].x + odd2[1].y);
       const unsigned again = __ballot_sync(0xffffffffu, live && !(odd == 0.f));
-      if (again) rows_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, again, seen, it.q0 + t, h, &dead_s[1]);
+      if (again && it.mode == kCareful)
+        rows_again<T, D, PAGED>(&a, &p, it.b, it.kh, it.k0, again, seen, it.q0 + t, h, &dead_s[1]);
+      else if (again && lane == 0)
+        flagged[(taken - 1) & 1] = 1;
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ tensor core
@@ -627,7 +687,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(leader, &s_full[i]);
     };
-    while (next()) {
+    // the products' arrivals at the barriers end before the CTA does, and its TMEM is given back; the softmax
+    // warps are at the last item's outputs meanwhile
+    unsigned drains = 0;
+    auto settle = [&]() {
+      commit(leader, &drained);
+      drain(&drained, drains++ & 1);
+      __syncwarp();
+    };
+    while (next(settle)) {
       const int seen[2] = {uniform(it.seen[0]), uniform(it.seen[1])}, len = uniform(it.len);
       const int j0 = uniform(it.j0), j1 = uniform(it.j1);
       const int tiles[2] = {min(tiles_of(seen[0]), j1), min(tiles_of(seen[1]), j1)};  // key tiles [j0, tiles[i])
@@ -684,16 +752,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j + 1 < j1) commit(leader, &kv_empty[kx % NS]);
       }
     }
-    commit(leader, &drained);  // before the TMEM is given back
-    drain(&drained, 0);
-    __syncwarp();
   } else if (warp == kZeroWarp) {
     // ------------------------------------------------------------------ behind the last value
     // What lies there is not this sequence's: zero, or its weight of zero would make NaN of a NaN.
     // v_tail says that the load of such a tile is under way (kv_full alone would not say which of the
     // stage's loads it speaks of), v_clean that it is ready; the stage is not loaded again before that.
     unsigned loads = 0, tails = 0;
-    while (next()) {
+    while (next([] {})) {
       const int rows = it.len - (it.j1 - 1) * kTile;
       if (it.j1 <= it.j0) continue;
       loads += 2 * (it.j1 - it.j0);
@@ -715,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ loads
     unsigned loads = 0, items[2] = {0, 0};
     const int rows_q = a.tok * a.rep;
-    while (next()) {
+    while (next([] {})) {
       const int* table = PAGED ? p.table + it.b * p.table_row : nullptr;
       for (int j = it.j0; j < it.j1; ++j) {
         for (int kv = 0; kv < 2; ++kv, ++loads) {
@@ -786,27 +851,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       return block;
     };
+    int w1 = -1, w2 = -1;  // the blocks of items n - 1 and n - 2
+    bool ended = SPLIT;    // there is no block to ask for
     for (unsigned n = 0;; ++n) {
-      int w = blockIdx.x, cut = 1;
-      if constexpr (SPLIT) {
-        cut = pieces<PAGED>(a, p, lane);
-        w = n ? -1 : w / cut;
-      } else if (n) {
+      int w = -1, cut = 1;
+      if constexpr (SPLIT) cut = pieces<PAGED>(a, p, lane);
+      it.mode = kItem;
+      if (n == 0) {
+        w = blockIdx.x / cut;
+      } else {
         wait_for(&item_empty, (n - 1) & 1, dead);
-        w = take();
-      }
-      it.none = w < 0 || !finder.find<PAGED>(a, p, lane, w, it);
-      if constexpr (!SPLIT) {
-        // Blocks without an item (sequences that are empty or fill their tiles leave some): taken too, each
-        // would begin as a CTA of its own only to end. Measured: 16 prompts and 1008 empty sequences 623 us
-        // without.
-        while (it.none && w >= 0) {
-          w = take();
-          it.none = w < 0 || !finder.find<PAGED>(a, p, lane, w, it);
+        if (flagged[n & 1]) {
+          w = w2;
+          it.mode = kCareful;
+          __syncwarp();
+          if (lane == 0 && !waited) flagged[n & 1] = 0;  // (behind last_flagged others may still have to read it)
         }
       }
+      bool none = w < 0 || !finder.find<PAGED>(a, p, lane, w, it);
+      // Blocks without an item (sequences that are empty or fill their tiles leave some): taken too, each
+      // would begin as a CTA of its own only to end. Measured: 16 prompts and 1008 empty sequences 623 us
+      // without.
+      while (none && !ended) {
+        w = take();
+        ended = w < 0;
+        none = ended || !finder.find<PAGED>(a, p, lane, w, it);
+      }
+      if (none) it.mode = kNone;
+      w2 = w1, w1 = w;
       if constexpr (SPLIT) {
-        if (n) wait_for(&item_empty, (n - 1) & 1, dead);
         const int piece = blockIdx.x - w * cut, tiles = it.j1;
         it.j0 = (int)((unsigned)tiles * piece / (unsigned)cut);  // at most 2^24 tiles x 148 pieces
         it.j1 = (int)((unsigned)tiles * (piece + 1) / (unsigned)cut);
@@ -825,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           j->cut = there ? cut : 0;
         }
       }
-      if (it.none) break;
+      if (none && (waited || !last_flagged(n - 1))) break;
     }
     if (*dead) drain(&answered, 0), drain(&answered, 1);
   }

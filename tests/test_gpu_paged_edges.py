@@ -125,3 +125,61 @@ def test_raised_keys_of_cut_items_are_weighed_against_one_another(cuda_device, d
         got = K.packed_attention(q, k, v, offsets([n], dev), offsets([keys], dev), causal=False, scale=rise)
         want, bound = oracle_rows(q, lambda b: (host(k), host(v)), [0, n], rise, False, dtype, UNIT[dtype])
         check(f"pieces, rise of {rise} at {raised} {dtype}", got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rise", [20.0, 100.0])
+@pytest.mark.parametrize("batch", [1, 40])  # cut along the keys, and not
+def test_scores_far_above_the_first_cost_no_more_than_others(cuda_device, dtype, rise, batch):
+    """Finite scores, however far apart, are no reason to compute rows again one by one: that would take a
+    thousand times as long as the call, where four times is allowed here."""
+    dev, d, n, heads, keys = cuda_device, 128, 40, 16, 2000
+    q = _first_element(dev, dtype, n * batch, heads, d)
+    cu, cu_k = offsets([n] * batch, dev), offsets([keys] * batch, dev)
+    v = normal(311, keys * batch, 1, d, dtype=dtype, device=dev)
+
+    def time_of(at):
+        k = torch.zeros(keys, 1, d, device=dev, dtype=dtype)
+        k[at:, 0, 0] = torch.arange(keys - at, device=dev).remainder(2).to(dtype)
+        k = k.repeat(batch, 1, 1)
+        best = float("inf")
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            K.packed_attention(q, k, v, cu, cu_k, causal=False, scale=rise)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    level = time_of(keys)  # no key is raised
+    for at in (1, 60, 100, 130, 500, 1990):
+        assert time_of(at) <= 4 * level + 0.05, (at, level)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("batch,longest", [(5, 2000), (400, 150)])
+def test_items_with_scores_far_apart_among_others(cuda_device, dtype, causal, batch, longest):
+    """Some sequences have keys far above their others, most have none: each gets what float64 gives it, and the
+    same bits from every call."""
+    dev, d, heads, rise = cuda_device, 64, 8, 100.0
+    r = np.random.default_rng(312)
+    new = [int(x) for x in r.integers(1, longest // 3, batch)]
+    lens = [n + int(x) for n, x in zip(new, r.integers(0, longest // 2, batch))]
+    q = _first_element(dev, dtype, sum(new), heads, d)
+    k = torch.zeros(sum(lens), 2, d, dtype=dtype)
+    at = np.concatenate(([0], np.cumsum(lens)))
+    for b in range(batch):
+        if b % 3 == 1:
+            for i in r.integers(0, lens[b], 3):
+                k[at[b] + i, int(r.integers(2)), 0] = float(r.choice([1.0, 0.9921875, 0.5, -1.0]))
+    k, v = k.to(dev), normal(313, sum(lens), 2, d, dtype=dtype, device=dev)
+    cu, cu_k = offsets(new, dev), offsets(lens, dev)
+    got = K.packed_attention(q, k, v, cu, cu_k, causal=causal, scale=rise)
+    for _ in range(5):
+        assert torch.equal(got, K.packed_attention(q, k, v, cu, cu_k, causal=causal, scale=rise))
+    hk, hv = host(k), host(v)
+    want, bound = oracle_rows(q, lambda b: (hk[at[b]:at[b + 1]], hv[at[b]:at[b + 1]]), np.concatenate(([0], np.cumsum(new))),
+                              rise, causal, dtype, UNIT[dtype])
+    check(f"far apart among others {dtype} causal {causal}", got, want, bound)
