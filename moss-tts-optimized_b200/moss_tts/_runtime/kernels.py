@@ -170,7 +170,9 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _DIMS = (64, 128)
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _current_device = torch.cuda.current_device
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the address alone, without a Stream object
+# the address alone, without a Stream object, where torch has the (private) function for it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _strides3(name, t, heads, d):
