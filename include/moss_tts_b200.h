@@ -384,8 +384,8 @@ typedef struct mt_paged_kv {
  * Head RMSNorm + rotate-half RoPE of packed new tokens, the query rows to q_out [tokens][nq][D] and
  * the key and value rows into their pages: qkv [tokens] rows of (nq + 2 heads) * D, qkv_row elements
  * apart. Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1])
- * and its last kv_lens[b] positions; cu_seqlens NULL: one token per sequence. Rows behind the last
- * sequence are left alone. q_norm / k_norm [D]; cos_tab / sin_tab [table_rows][D] in the cache's type,
+ * and its last kv_lens[b] positions; cu_seqlens NULL: one token per sequence, none for a sequence of length 0
+ * (an empty slot: zeros in its query row, no error). Rows behind the last sequence are left alone. q_norm / k_norm [D]; cos_tab / sin_tab [table_rows][D] in the cache's type,
  * or fp32 with table_fp32. All arithmetic is fp32 with one rounding at the store (mt_qk_rope_kv rounds
  * after every step, as the reference does). A page that is written belongs to one sequence.
  */

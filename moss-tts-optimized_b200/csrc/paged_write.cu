@@ -55,6 +55,15 @@ __global__ void __launch_bounds__(kThreads) qk_rope_paged(WriteArgs a, Pages p) 
   const int b = a.cu ? sequence_of(a.cu, p.batch, t, lane) : t;
   if (b >= p.batch || (a.cu && a.cu[b] > t)) return;  // behind the last sequence
   const int len = p.lens[b];
+  char* qo = a.q_out + ((long long)t * a.nq * D + sub * 8) * 2;
+  if (!a.cu && len == 0) {  // an empty slot of a step: no token, so zeros for its query and nothing in the pages
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int h = h0 + n * kGroups + group;
+      if (h < a.nq) *reinterpret_cast<uint4*>(qo + (long long)h * D * 2) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
   const int pos = a.cu ? len - a.cu[b + 1] + t : len - 1;
   if (pos < 0 || pos >= a.table_rows || (pos >> p.shift) >= p.max_pages) {
     if (a.status && threadIdx.x == 0) atomicExch(a.status, kStatusPosition);
@@ -86,7 +95,6 @@ __global__ void __launch_bounds__(kThreads) qk_rope_paged(WriteArgs a, Pages p) 
   const float sign = sub < kLanes / 2 ? -1.f : 1.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] *= sign;
-  char* qo = a.q_out + ((long long)t * a.nq * D + sub * 8) * 2;
   char* ko = p.k + (page * p.k_page + slot * p.k_row + sub * 8) * 2;
   char* vo = p.v + (page * p.v_page + slot * p.v_row + sub * 8) * 2;
 #pragma unroll

@@ -299,8 +299,9 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     ``page_table[b, j // page_size]`` (int32 ``[batch, max_pages]``) of ``k_pages`` / ``v_pages``
     ``[pages, nkv, page_size, D]`` (any strides with adjacent D; page_size a power of two, 16 to 256; D 64 or
     128). ``kv_lens`` int32 ``[batch]`` counts each sequence's tokens with the new ones; ``cu_seqlens`` int32
-    ``[batch + 1]`` are the new tokens' offsets in ``qkv``, or None for one token per sequence. Returns the
-    rotated queries ``[tokens, nq, D]`` (in ``out`` if given, which has memory of its own); rows behind the last
+    ``[batch + 1]`` are the new tokens' offsets in ``qkv``, or None for one token per sequence, where a sequence
+    of length 0 is an empty slot: zeros in its query row, nothing in the pages. Returns the rotated queries
+    ``[tokens, nq, D]`` (in ``out`` if given, which has memory of its own); rows behind the last
     sequence are not written.
 
     Unlike ``qk_rope_decode``, whose intermediate roundings are the reference's, this rounds once, at the

@@ -4,9 +4,10 @@ import numpy as np
 import pytest
 import torch
 
-from paged_cases import UNIT, check, host, normal, offsets, oracle_rows
+from paged_cases import UNIT, check, host, ints, make_cache, normal, offsets, oracle_rows
 
 from moss_tts._runtime import kernels as K, native
+from moss_tts._runtime.engine import rope_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +184,48 @@ def test_items_with_scores_far_apart_among_others(cuda_device, dtype, causal, ba
     want, bound = oracle_rows(q, lambda b: (hk[at[b]:at[b + 1]], hv[at[b]:at[b + 1]]), np.concatenate(([0], np.cumsum(new))),
                               rise, causal, dtype, UNIT[dtype])
     check(f"far apart among others {dtype} causal {causal}", got, want, bound)
+
+
+# ------------------------------------------------------------------------------------ slots without a sequence
+@pytest.mark.parametrize("dtype,nq,nkv,d,page", [(BF, 32, 8, 128, 64), (HF, 3, 1, 64, 16), (BF, 7, 1, 64, 256)])
+@pytest.mark.parametrize("lens", [[0, 40], [0], [5, 0, 0, 33, 0]])
+def test_a_step_with_empty_slots(cuda_device, dtype, nq, nkv, d, page, lens):
+    """A padded decode step: a slot of length 0 is no error to the write, its query row is zeros whatever its
+    q | k | v holds, no page changes for it, and the attention gives zeros; the others are as without it."""
+    dev = cuda_device
+    live = [b for b, n in enumerate(lens) if n]
+    kp, vp, table = make_cache(340, lens, nkv, d, page, dtype, dev)
+    qkv = normal(341, len(lens), (nq + 2 * nkv) * d, dtype=dtype, device=dev)
+    qkv[[b for b, n in enumerate(lens) if not n]] = float("nan")
+    w = torch.ones(d, device=dev, dtype=dtype)
+    cos, sin = (t.to(dev) for t in rope_tables(64, d))
+    cos, sin = cos.to(dtype), sin.to(dtype)
+    alone = kp.clone(), vp.clone()
+    ln, status = ints(lens, dev), ints([0], dev)
+    out = torch.full((len(lens), nq, d), 7.0, device=dev, dtype=dtype)
+    q = K.qk_rope_paged(qkv, w, w, cos, sin, kp, vp, table, ln, None, 1e-6, out=out, status=status)
+    assert int(status.item()) == 0
+    assert all(bool((q[b] == 0).all()) for b in range(len(lens)) if b not in live)
+    if live:
+        want = K.qk_rope_paged(qkv[live], w, w, cos, sin, *alone, table[live], ln[live], None, 1e-6)
+        assert torch.equal(q[live], want)
+    assert torch.equal(kp.nan_to_num(9.0), alone[0].nan_to_num(9.0))
+    assert torch.equal(vp.nan_to_num(9.0), alone[1].nan_to_num(9.0))
+    got = K.paged_attention_decode(q, kp, vp, table, ln, status=status)
+    assert int(status.item()) == 0 and bool(torch.isfinite(got).all())
+    assert all(bool((got[b] == 0).all()) for b in range(len(lens)) if b not in live)
+
+
+def test_a_position_outside_the_tables_is_still_said(cuda_device):
+    """What is an error beside an empty slot: a length beyond the tables, a negative one, and a token that
+    offsets give to a sequence of length 0."""
+    dev, nq, nkv, d = cuda_device, 4, 2, 128
+    kp, vp, table = make_cache(342, [40, 40], nkv, d, 16, BF, dev, rubbish=0.5)
+    qkv, w = normal(343, 2, (nq + 2 * nkv) * d, device=dev), torch.ones(d, device=dev, dtype=BF)
+    cos, sin = (t.to(dev).to(BF) for t in rope_tables(64, d))
+    before = kp.clone(), vp.clone()
+    for lens, cu in (([49, 0], None), ([0, 49], None), ([0, -1], None), ([0, 0], offsets([1, 1], dev))):
+        status = ints([0], dev)
+        K.qk_rope_paged(qkv, w, w, cos, sin, kp, vp, table, ints(lens, dev), cu, 1e-6, status=status)
+        assert int(status.item()) == 1
+        assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
