@@ -364,7 +364,8 @@ int mt_prefill_attention(const void* q, const void* k_cache, const void* v_cache
  * tokens of each sequence, the new ones included. type 0 = bf16, 1 = fp16; head_dim 64 or 128;
  * page_size a power of two, 16 to 256; 16-byte aligned pages. The struct itself is read on the host
  * during the call.
- * No output of the calls below shares memory with an input.
+ * No output of the calls below shares memory with an input: a call whose output begins before an input's last
+ * byte and ends behind its first is refused.
  * `status` (int32, may be NULL) takes 1 where a length exceeds the page table or a position the rope
  * tables, 3 where a page id lies outside the cache. A bad length is cut to what the table holds; a
  * bad page reads as zeros and is not written; a bad position writes nothing.

@@ -4,6 +4,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace mt {
@@ -195,6 +197,34 @@ static inline bool pages_of(const mt_paged_kv* kv, Pages* p) {
   p->shift = __builtin_ctz((unsigned)kv->page_size);
   p->max_pages = kv->max_pages;
   p->batch = kv->batch;
+  return true;
+}
+
+// Host: the bytes from an operand's first element to its last.
+struct Span {
+  const char *first, *past;
+};
+static inline Span span_of_bytes(const void* p, long long bytes) { return {(const char*)p, (const char*)p + (p ? bytes : 0)}; }
+// Rows of heads of d 16-bit elements.
+static inline Span span_of_rows(const void* p, long long rows, long long row, long long heads, long long head, int d) {
+  return span_of_bytes(p, 2 * ((rows - 1) * row + (heads - 1) * head + d));
+}
+static inline Span span_of_pages(const mt_paged_kv* kv, bool values) {
+  const long long last = values ? (kv->pages - 1) * kv->v_page_stride + (kv->heads - 1) * kv->v_head_stride +
+                                      (kv->page_size - 1) * kv->v_row_stride
+                                : (kv->pages - 1) * kv->k_page_stride + (kv->heads - 1) * kv->k_head_stride +
+                                      (kv->page_size - 1) * kv->k_row_stride;
+  return span_of_bytes(values ? kv->v_pages : kv->k_pages, 2 * (last + kv->head_dim));
+}
+static inline Span span_of_table(const mt_paged_kv* kv) {
+  return span_of_bytes(kv->page_table, 4 * ((kv->batch - 1) * kv->table_stride + kv->max_pages));
+}
+static inline Span span_of_ints(const void* p, long long n) { return span_of_bytes(p, 4 * n); }
+// Whether what is written lies apart from all that is read: rows are read by other blocks than the one that
+// writes them, and some a second time.
+static inline bool apart(Span written, std::initializer_list<Span> read) {
+  for (const Span& r : read)
+    if (r.first < written.past && written.first < r.past) return false;
   return true;
 }
 

@@ -545,6 +545,11 @@ MT_API int mt_paged_attention_decode(const void* q, int q_row, int q_head, const
   if (q_row < 1 || q_head < 1 || q_row % 8 || q_head % 8 || !aligned(q, 16) || !aligned(out, 16) ||
       !aligned(workspace, 16))
     return kBadArgument;
+  const int d = kv->head_dim;
+  if (!paged::apart(paged::span_of_rows(out, kv->batch, (long long)nq * d, nq, d, d),
+                    {paged::span_of_rows(q, kv->batch, q_row, nq, q_head, d), paged::span_of_pages(kv, false),
+                     paged::span_of_pages(kv, true), paged::span_of_table(kv), paged::span_of_ints(kv->kv_lens, kv->batch)}))
+    return kBadArgument;
   const int rep = nq / kv->heads, groups = (rep + paged::kHeads - 1) / paged::kHeads;
   const long long items = (long long)kv->batch * kv->heads * groups;
   const long long most = items * (((long long)kv->max_pages * kv->page_size + paged::kChunk - 1) / paged::kChunk);

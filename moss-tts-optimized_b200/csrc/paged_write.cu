@@ -165,6 +165,18 @@ MT_API int mt_qk_rope_paged(const void* qkv, const void* q_norm, const void* k_n
   const void* wide[6] = {qkv, q_norm, k_norm, cos_tab, sin_tab, q_out};
   for (const void* x : wide)
     if (!aligned(x, 16)) return kBadArgument;
+  const int d = kv->head_dim;
+  const long long table = (long long)table_rows * d * (table_fp32 ? 4 : 2);
+  const paged::Span pages[2] = {paged::span_of_pages(kv, false), paged::span_of_pages(kv, true)};
+  const paged::Span rows = paged::span_of_rows(q_out, tokens, (long long)nq * d, nq, d, d);
+  for (const paged::Span& written : {rows, pages[0], pages[1]})
+    if (!paged::apart(written, {paged::span_of_bytes(qkv, 2 * ((tokens - 1LL) * qkv_row + (nq + 2LL * kv->heads) * d)),
+                                paged::span_of_bytes(q_norm, 2 * d), paged::span_of_bytes(k_norm, 2 * d),
+                                paged::span_of_bytes(cos_tab, table), paged::span_of_bytes(sin_tab, table),
+                                paged::span_of_table(kv), paged::span_of_ints(kv->kv_lens, kv->batch),
+                                paged::span_of_ints(cu_seqlens, kv->batch + 1LL)}))
+      return kBadArgument;
+  if (!paged::apart(rows, {pages[0], pages[1]})) return kBadArgument;
   const paged::WriteArgs a{(const char*)qkv,     (const char*)q_norm, (const char*)k_norm, (const char*)cos_tab,
                            (const char*)sin_tab, (const int*)cu_seqlens, (char*)q_out,   (int*)status,
                            qkv_row,              tokens,              nq,                  table_rows,

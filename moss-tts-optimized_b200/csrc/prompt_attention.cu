@@ -1089,6 +1089,12 @@ MT_API int mt_packed_attention(const void* q, int q_row, int q_head, const void*
   if (k_row < 1 || k_head < 1 || v_row < 1 || v_head < 1 || k_row % 8 || k_head % 8 || v_row % 8 || v_head % 8 ||
       !aligned(k, 16) || !aligned(v, 16) || !aligned(cu_k, 4) || !aligned(workspace, 32))
     return kBadArgument;
+  if (!paged::apart(paged::span_of_rows(out, tokens_q, (long long)nq * head_dim, nq, head_dim, head_dim),
+                    {paged::span_of_rows(q, tokens_q, q_row, nq, q_head, head_dim),
+                     paged::span_of_rows(k, tokens_k, k_row, nkv, k_head, head_dim),
+                     paged::span_of_rows(v, tokens_k, v_row, nkv, v_head, head_dim),
+                     paged::span_of_ints(cu_q, batch + 1LL), paged::span_of_ints(cu_k, batch + 1LL)}))
+    return kBadArgument;
   const int rep = nq / nkv;
   prompt::PromptArgs a{(const char*)q, (const char*)k, (const char*)v, (char*)out, (const int*)cu_q,
                        (const int*)cu_k, nullptr, q_row, q_head, k_row, k_head, v_row, v_head,
@@ -1105,6 +1111,12 @@ MT_API int mt_paged_attention_prompt(const void* q, int q_row, int q_head, const
   paged::Pages p;
   if (!paged::pages_of(kv, &p) || !prompt::query_ok(q, q_row, q_head, cu_seqlens, tokens, nq, kv->heads, out) ||
       !aligned(workspace, 32))
+    return kBadArgument;
+  const int d = kv->head_dim;
+  if (!paged::apart(paged::span_of_rows(out, tokens, (long long)nq * d, nq, d, d),
+                    {paged::span_of_rows(q, tokens, q_row, nq, q_head, d), paged::span_of_pages(kv, false),
+                     paged::span_of_pages(kv, true), paged::span_of_table(kv), paged::span_of_ints(kv->kv_lens, kv->batch),
+                     paged::span_of_ints(cu_seqlens, kv->batch + 1LL)}))
     return kBadArgument;
   const int rep = nq / kv->heads;
   prompt::PromptArgs a{(const char*)q, nullptr, nullptr, (char*)out, (const int*)cu_seqlens, nullptr, (int*)status,

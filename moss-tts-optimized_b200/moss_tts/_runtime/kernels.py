@@ -230,13 +230,30 @@ def _out(out, shape, like):
             or not out.is_contiguous() or out.data_ptr() & 31:
         raise ValueError(f"out must be a contiguous, 32-byte aligned {like.dtype} tensor {tuple(shape)} on the "
                          "queries' device")
-    # rows are read by other blocks than the one that writes them, and some a second time
-    if out.numel() and like.numel():
-        at, first = out.data_ptr(), like.data_ptr()
-        if at < first + 2 * (1 + sum((n - 1) * x for n, x in zip(like.shape, like.stride()))) \
-                and first < at + 2 * out.numel():
-            raise ValueError("out must not lie in the queries' memory")
     return out
+
+
+def _extent(t):
+    """The addresses of a tensor's first byte and behind its last."""
+    first = t.data_ptr()
+    if not t.numel():
+        return first, first
+    n = 1
+    for size, stride in zip(t.shape, t.stride()):
+        n += (size - 1) * stride
+    return first, first + n * t.element_size()
+
+
+def _apart(written, read):
+    """Says which output lies in an input's memory, where that is what an entry point has refused: rows are read
+    by other blocks than the one that writes them, and some a second time."""
+    for name, w in written.items():
+        first, past = _extent(w)
+        for other, t in (written | read).items():
+            # (keys and values may lie side by side)
+            if t is not None and name != other and {name, other} != {"k_pages", "v_pages"} \
+                    and _extent(t)[0] < past and _extent(t)[1] > first:
+                raise ValueError(f"{name} must not lie in the memory of {other}")
 
 
 def _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev):
@@ -273,18 +290,23 @@ def _paged(k_pages, v_pages, page_table, kv_lens, dtype, dev):
                                 vr, row, pages, heads, size, d, most, batch, _TYPES[dtype]), batch, most * size
 
 
-def _call_on(dev, name, *args, workspace=None):
+def _call_on(dev, name, *args, workspace=None, apart=None):
     """``native.call`` on device ``dev`` and its current stream; ``workspace`` (function, arguments) gives the
     bytes of a workspace, which comes last before the status, flags and stream. It is taken from torch's
-    allocator for the one call, so that calls on other streams and captured graphs have one each."""
+    allocator for the one call, so that calls on other streams and captured graphs have one each. ``apart()``
+    gives the tensors that are written and those that are read, by name, for a call that is refused."""
     if _current_device() != dev:
         with torch.cuda.device(dev):
-            return _call_on(dev, name, *args, workspace=workspace)
+            return _call_on(dev, name, *args, workspace=workspace, apart=apart)
     if workspace is not None:
         n = workspace[0](*workspace[1:])
         held = torch.empty(n, device=torch.device("cuda", dev), dtype=torch.uint8) if n else None
         args = [held.data_ptr() if a is _WORKSPACE and n else None if a is _WORKSPACE else a for a in args]
-    native.call(name, *args, _raw_stream(dev))
+    try:
+        native.call(name, *args, _raw_stream(dev))
+    except RuntimeError:
+        _apart(*apart())
+        raise
 
 
 _WORKSPACE = object()  # stands for the workspace's address in _call_on's arguments
@@ -344,7 +366,10 @@ def qk_rope_paged(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_tabl
     if tokens:
         _call_on(dev, "mt_qk_rope_paged", qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(),
                  sin.data_ptr(), table[0], 1 if kind is torch.float32 else 0, kv, cu, tokens, nq, row, out.data_ptr(),
-                 eps, st, 0)
+                 eps, st, 0,
+                 apart=lambda: ({"out": out, "k_pages": k_pages, "v_pages": v_pages},
+                                {"qkv": qkv, "q_weight": q_weight, "k_weight": k_weight, "cos": cos, "sin": sin,
+                                 "page_table": page_table, "kv_lens": kv_lens, "cu_seqlens": cu_seqlens}))
     return out
 
 
@@ -367,7 +392,9 @@ def paged_attention_decode(q, k_pages, v_pages, page_table, kv_lens, *, scale=No
     st = _status(status, dev)
     out = _out(out, (batch, nq, d), q)
     _call_on(dev, "mt_paged_attention_decode", q.data_ptr(), row, head, kv, nq, d ** -0.5 if scale is None else scale,
-             out.data_ptr(), _WORKSPACE, st, 0, workspace=(native.paged_decode_workspace, dev))
+             out.data_ptr(), _WORKSPACE, st, 0, workspace=(native.paged_decode_workspace, dev),
+             apart=lambda: ({"out": out}, {"the queries": q, "k_pages": k_pages, "v_pages": v_pages,
+                                           "page_table": page_table, "kv_lens": kv_lens}))
     return out
 
 
@@ -407,7 +434,9 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=True, s
     _call_on(dev, "mt_packed_attention", q.data_ptr(), row, head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
              v_head, cu_q, cu_k, batch, tokens, tokens_k, nq, nkv, d, _TYPES[dtype], 1 if causal else 0,
              d ** -0.5 if scale is None else scale, out.data_ptr(), _WORKSPACE, 0,
-             workspace=(native.prompt_workspace, tokens, batch, tokens_k, nq, nkv, d))
+             workspace=(native.prompt_workspace, tokens, batch, tokens_k, nq, nkv, d),
+             apart=lambda: ({"out": out}, {"the queries": q, "k": k, "v": v, "cu_seqlens_q": cu_seqlens_q,
+                                           "cu_seqlens_k": cu_seqlens_k}))
     return out
 
 
@@ -429,5 +458,7 @@ def paged_attention_prompt(q, k_pages, v_pages, page_table, kv_lens, cu_seqlens,
     if tokens:
         _call_on(dev, "mt_paged_attention_prompt", q.data_ptr(), row, head, kv, cu, tokens, nq,
                  d ** -0.5 if scale is None else scale, out.data_ptr(), _WORKSPACE, st, 0,
-                 workspace=(native.prompt_workspace, tokens, batch, most, nq, nkv, d))
+                 workspace=(native.prompt_workspace, tokens, batch, most, nq, nkv, d),
+                 apart=lambda: ({"out": out}, {"the queries": q, "k_pages": k_pages, "v_pages": v_pages,
+                                               "page_table": page_table, "kv_lens": kv_lens, "cu_seqlens": cu_seqlens}))
     return out

@@ -229,3 +229,37 @@ def test_a_position_outside_the_tables_is_still_said(cuda_device):
         K.qk_rope_paged(qkv, w, w, cos, sin, kp, vp, table, ints(lens, dev), cu, 1e-6, status=status)
         assert int(status.item()) == 1
         assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+
+
+# ------------------------------------------------------------------------------------ memory of inputs
+def test_outputs_in_the_memory_of_keys_values_and_pages_are_refused(cuda_device):
+    dev, nq, nkv, d, page = cuda_device, 4, 2, 64, 16
+    pool = normal(350, 2, 8, nkv, page, d, device=dev)  # keys and values
+    kp, vp = pool[0], pool[1]
+    table, ln, cu = ints([[0, 1], [2, 3]], dev), ints([20, 3], dev), offsets([1, 1], dev)
+    q = normal(351, 2, nq, d, device=dev)
+    qkv, w = normal(352, 2, (nq + 2 * nkv) * d, device=dev), torch.ones(d, device=dev, dtype=BF)
+    cos, sin = (t.to(dev).to(BF) for t in rope_tables(32, d))
+    before = pool.clone()
+    flat = pool.view(-1)
+    for first in (0, 4096, pool[0].numel() + 64):
+        out = flat[first:first + q.numel()].view(q.shape)
+        for call in (lambda: K.paged_attention_decode(q, kp, vp, table, ln, out=out),
+                     lambda: K.paged_attention_prompt(q, kp, vp, table, ln, cu, out=out),
+                     lambda: K.qk_rope_paged(qkv, w, w, cos, sin, kp, vp, table, ln, None, 1e-6, out=out)):
+            with pytest.raises(ValueError, match="memory"):
+                call()
+    rows = normal(353, 12, nq + 2 * nkv, d, device=dev)
+    k, v = rows[4:, nq:nq + nkv], rows[4:, nq + nkv:]
+    cu_k = ints([0, 3, 5], dev)
+    for first, ends in ((4, True), (10, True), (0, False)):  # whole rows, k and v among them
+        out = rows.view(-1)[first * rows.stride(0):][:q.numel()].view(q.shape)
+        if ends:
+            with pytest.raises(ValueError, match="memory"):
+                K.packed_attention(q, k, v, cu, cu_k, out=out)
+        else:
+            K.packed_attention(q, k, v, cu, cu_k, out=out)
+    inside = flat[:qkv.numel()].view(qkv.shape)
+    with pytest.raises(ValueError, match="memory"):
+        K.qk_rope_paged(inside, w, w, cos, sin, kp, vp, table, ln, None, 1e-6)
+    assert torch.equal(pool, before)
