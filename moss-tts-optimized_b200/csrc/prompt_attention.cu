@@ -21,8 +21,8 @@
 // special-function unit, one exponential a score; it takes 3270, for each tile goes round a chain that
 // nothing shortens: scores seen 300 cycles after their product, weights 1840, seen by the issuing lane 250
 // to 400, products 790. Measured, bf16, 32 query and 8 key heads of 128, in a graph: 8191 causal tokens
-// 432 us (1.27 PFLOP/s; 507 us under the power cap of minutes of it), 16 prompts of 1 to 1024 tokens 86 us,
-// 48 tokens behind 16001 keys 34 us. Tried and slower: two issuing warps (545 us: the tiles fall into step
+// 422 us (1.30 PFLOP/s; 490 us under the power cap of minutes of it), 16 prompts of 1 to 1024 tokens 85 us,
+// 48 tokens behind 16001 keys 33 us; fp16 541, 106 and 40 us, for its weights go out all at once. Tried and slower: two issuing warps (545 us: the tiles fall into step
 // and meet at either unit), sixteen softmax warps with two threads a row (441), a part of the exponentials
 // by polynomial (470: packed fp32 instructions take two issue slots), the output turned through shared
 // memory (16 prompts 96 us), all weights announced at once (432 against 426), the maximum of every
@@ -55,9 +55,12 @@ constexpr int kTmemCols = 512;
 constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
 // Softmax weights round to the values' type for the tensor core, by 2^-9 of themselves on average for bf16:
 // with the rounding of the output that makes an error sqrt(2) times the output's alone. Calls of up to
-// kFineRows rows, single tokens for most, are as exact as the decode kernel (FINE): a weight is the sum of two
-// 16-bit numbers, the second in the other half of the scores' columns. Measured in a graph: 33 tokens of 32
-// heads 7.2 us without and 8.2 with, 48 rows behind 16001 keys 34 and 41 us, hence not for more rows.
+// kFineRows rows (tokens_q * nq, rows of no sequence counted), single tokens for most, are as exact as the decode kernel (FINE): a weight is the sum of two
+// 16-bit numbers, the second in the other half of the scores' columns. Measured in a graph, 32 heads,
+// one number and two, bf16 (fp16): 16 tokens (512 rows) 7.0 and 8.2 us (7.5, 9.4), 24 tokens 7.4 and 8.6 (7.7, 9.6),
+// one token of 16 sequences of 2000 keys 30 and 43 (37, 65), of 24 sequences 55 and 78 (66, 122), 48 tokens
+// behind 16001 keys 30 and 37 (33, 49). A call of single tokens is the decode kernel's; larger ones are not made
+// to pay a quarter to four fifths more for it.
 //
 // The reference m that a row's exponentials are taken against need not be the largest score: weights far
 // above 1 lose nothing in fp32 sums and 16-bit floating weights. It begins at the row's first score and

@@ -263,3 +263,34 @@ def test_outputs_in_the_memory_of_keys_values_and_pages_are_refused(cuda_device)
     with pytest.raises(ValueError, match="memory"):
         K.qk_rope_paged(inside, w, w, cos, sin, kp, vp, table, ln, None, 1e-6)
     assert torch.equal(pool, before)
+
+
+def test_second_passes_in_a_graph_and_on_two_streams(cuda_device):
+    """Items that go round again, captured once and replayed on two streams at once, whole and cut: the bits of
+    the plain calls, and no wait expires."""
+    dev, d, heads, rise = cuda_device, 128, 8, 120.0
+    native.error_word(clear=True)
+    sides = []
+    for side, (new, lens) in enumerate((([60, 1, 300], [900, 700, 300]), ([40], [3000]))):
+        q = normal(360 + side, sum(new), heads, d, device=dev) * 0.01
+        q[..., 0] = 1
+        k, v = normal(362 + side, sum(lens), 1, d, device=dev) * 0.01, normal(364 + side, sum(lens), 1, d, device=dev)
+        k[..., 0] = 0
+        k[5::97, :, 0] = 1
+        cu, cu_k = offsets(new, dev), offsets(lens, dev)
+        plain = K.packed_attention(q, k, v, cu, cu_k, scale=rise)
+        out, stream, graph = torch.zeros_like(q), torch.cuda.Stream(dev), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize(dev)
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(3):
+                K.packed_attention(q, k, v, cu, cu_k, scale=rise, out=out)
+        sides.append((plain, out, stream, graph, (q, k, v, cu, cu_k)))
+    for _ in range(20):
+        for _, out, stream, graph, _ in sides:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+    torch.cuda.synchronize(dev)
+    assert native.error_word() == 0
+    for plain, out, *_ in sides:
+        assert bool(torch.isfinite(plain).all()) and torch.equal(plain, out)
