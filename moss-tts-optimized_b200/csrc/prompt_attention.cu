@@ -55,12 +55,12 @@ constexpr int kTmemCols = 512;
 constexpr unsigned long long kDeadlineNs = 4000ull * 1000 * 1000;
 // Softmax weights round to the values' type for the tensor core, by 2^-9 of themselves on average for bf16:
 // with the rounding of the output that makes an error sqrt(2) times the output's alone. Calls of up to
-// kFineRows rows (tokens_q * nq, rows of no sequence counted), single tokens for most, are as exact as the decode kernel (FINE): a weight is the sum of two
-// 16-bit numbers, the second in the other half of the scores' columns. Measured in a graph, 32 heads,
-// one number and two, bf16 (fp16): 16 tokens (512 rows) 7.0 and 8.2 us (7.5, 9.4), 24 tokens 7.4 and 8.6 (7.7, 9.6),
-// one token of 16 sequences of 2000 keys 30 and 43 (37, 65), of 24 sequences 55 and 78 (66, 122), 48 tokens
-// behind 16001 keys 30 and 37 (33, 49). A call of single tokens is the decode kernel's; larger ones are not made
-// to pay a quarter to four fifths more for it.
+// kFineRows rows (tokens_q * nq, rows of no sequence counted), single tokens for most, are as exact as the
+// decode kernel (FINE): a weight is the sum of two 16-bit numbers, the second in the other half of the scores'
+// columns. Measured in a graph, 32 heads, one number and two, bf16 (fp16): 16 tokens (512 rows) 7.0 and 8.2 us
+// (7.5, 9.4), 24 tokens 7.4 and 8.6 (7.7, 9.6), one token of 16 sequences of 2000 keys 30 and 43 (37, 65), of 24
+// sequences 55 and 78 (66, 122), 48 tokens behind 16001 keys 30 and 37 (33, 49). Single tokens have the decode
+// kernel for speed; larger calls are not made to pay a sixth to four fifths more.
 //
 // The reference m that a row's exponentials are taken against need not be the largest score: weights far
 // above 1 lose nothing in fp32 sums and 16-bit floating weights. It begins at the row's first score and
